@@ -280,6 +280,113 @@ int nvfp4_quantize(const void* x, int32_t x_is_bf16, void* packed, void* sf_plai
 int nvfp4_gemm_static_scratch(const nvfp4_problem* problem, int workers, void* stream);
 
 /*
+ * ---- Mixture of experts: routing, the experts' products, the way back ----
+ *
+ * A token takes top_k of `experts` experts; pair (t, j) is its j-th choice.  The pairs are brought into EXPERT ORDER (by expert,
+ * within an expert by token and choice), and everything between the router and the combination works on one row
+ * per pair in that order.  The reference has no counterpart (one dense product).
+ *
+ * nvfp4_routing is the result of the router on the device; all its memory is the caller's, and none of these
+ * functions keeps anything of a call.  Sizes come from nvfp4_routing_plan().  Not more than 1024 experts, 32 choices and
+ * 2^31 - 1 pairs; tokens may be 0.
+ */
+typedef struct nvfp4_routing {
+    int32_t tokens, top_k, experts;
+    int32_t* expert; /* [tokens][top_k] the choices; -1: none (fewer experts were available) */
+    int32_t* row;    /* [tokens][top_k] row of the pair in expert order; -1: none */
+    int32_t* offset; /* [experts + 1] first row of each expert, then the number of rows */
+    void* plan;      /* plan_bytes, 16-byte aligned: the tiles that the grouped product walks (opaque) */
+} nvfp4_routing;
+
+/*
+ * plan_bytes: size of nvfp4_routing.plan.  sf_rows: the scales of a routed operand (nvfp4_quantize_routed, the NVFP4 output of
+ * nvfp4_expert_gemm) take sf_rows * (k / 16) bytes.  tile_tokens: rows of an expert that the grouped product takes
+ * at a time (32, or 256 from 16 rows per expert on average).  Any of them may be NULL.
+ */
+int nvfp4_routing_plan(int32_t tokens, int32_t top_k, int32_t experts, int32_t* tile_tokens, int64_t* plan_bytes, int64_t* sf_rows);
+
+/*
+ * The router.  s_e = softmax over the experts, or sigmoid, of the logits; choice c_e = s_e + bias[e] (without bias and with groups
+ * judged by their best the order is that of the logits themselves: both functions keep it).  With groups > 1 the experts fall into
+ * `groups` equal ranges, a range is judged by the sum of its group_top (1 or 2) largest c_e, and experts outside the top_groups best ranges
+ * are out.  The top_k largest c_e are taken, largest first, ties to the lowest index (of groups too);
+ * weights[t][j] = s of the choice, divided by their sum if renormalize (0 where that is 0), times scale.
+ * An expert whose logit or bias is -inf or NaN cannot be chosen; +inf counts as the largest number.  Where fewer than
+ * top_k can, the rest are expert -1, row -1, weight 0.  Choices are made in 64 bits: they do not depend on how a
+ * 32-bit sigmoid rounds.
+ */
+#define NVFP4_SCORE_SOFTMAX 0
+#define NVFP4_SCORE_SIGMOID 1
+#define NVFP4_LOGITS_FP16 0
+#define NVFP4_LOGITS_BF16 1
+#define NVFP4_LOGITS_FP32 2
+typedef struct nvfp4_router {
+    const void* logits;         /* [tokens][experts] */
+    int32_t logits_type;        /* NVFP4_LOGITS_* */
+    int64_t logits_row_stride;  /* elements */
+    const float* bias;          /* [experts] or NULL */
+    int32_t scoring;            /* NVFP4_SCORE_* */
+    int32_t groups, top_groups; /* 1, 1: no groups; up to 32, experts a multiple of groups */
+    int32_t group_top;          /* 1 or 2 */
+    int32_t renormalize;
+    float scale;
+    float* weights;             /* [tokens][top_k] */
+} nvfp4_router;
+int nvfp4_route(const nvfp4_router* router, const nvfp4_routing* routing, void* stream);
+
+/* The order of the pairs alone, for choices made elsewhere: routing->expert is read (what is not an expert counts as none; the
+ * same expert twice in a token gives two rows), the rest is written. */
+int nvfp4_plan_experts(const nvfp4_routing* routing, void* stream);
+
+/*
+ * Token rows x (fp16, or bf16 if x_is_bf16; [tokens][k], 16-byte aligned, stride in elements a multiple of 8) -> NVFP4 rows in expert
+ * order: packed [tokens * top_k][k / 2] and sf.  A token is quantised once, by the rule of nvfp4_quantize(), and
+ * written to each of its rows.  k a multiple of 64.
+ */
+int nvfp4_quantize_routed(const void* x, int32_t x_is_bf16, int64_t x_row_stride, int32_t k, const nvfp4_routing* routing, void* packed,
+                          int64_t packed_row_stride, void* sf, void* stream);
+
+/*
+ * The experts' product: row r of expert e in expert order,
+ *   z[r][n] = alpha[e] * sum_k A[r][k] W[e][n][k] + bias[e][n]
+ *   out     = out_scale * act(z): none, relu, silu, or (NVFP4_ACT_SWIGLU) silu(z_gate) * z_up with n / 2 columns: gate and up
+ *             rows of W alternate in groups of eight (eight gate rows, the eight up rows of the same columns, ...)
+ * as fp16 [tokens * top_k][n_out], or (NVFP4_OUT_NVFP4) re-quantised like nvfp4_gemm_epilogue() does, as the routed operand of a following
+ * product with k = n_out.  Rows from offset[experts] on are left as they were.  W and its scales are laid out like b and sfb_perm of
+ * nvfp4_problem with one batch entry per expert.  n % 128 == 0, k % 256 == 0, pointers and strides 16-byte aligned.
+ */
+#define NVFP4_ACT_SWIGLU 3
+typedef struct nvfp4_expert_problem {
+    const void* a;          /* packed rows in expert order */
+    const void* sfa;        /* their scales, as nvfp4_quantize_routed() writes them */
+    const void* w;
+    const void* sfw_perm;
+    const float* alpha;     /* [experts] or NULL (1) */
+    const void* bias;       /* fp16 [experts][n] or NULL */
+    int32_t n, k;
+    int64_t a_row_stride;                     /* bytes */
+    int64_t w_row_stride, w_expert_stride;    /* bytes */
+    int64_t sfw_perm_expert_stride;           /* bytes */
+    int64_t bias_expert_stride;               /* elements */
+    int32_t activation;     /* NVFP4_ACT_* */
+    int32_t output;         /* NVFP4_OUT_* */
+    float out_scale;
+    void* out;              /* fp16 or packed e2m1 */
+    int64_t out_row_stride; /* fp16: elements; NVFP4: bytes */
+    void* out_sf;           /* NVFP4: scales, sf_rows * (n_out / 16) bytes */
+} nvfp4_expert_problem;
+int nvfp4_expert_gemm(const nvfp4_expert_problem* problem, const nvfp4_routing* routing, void* stream);
+
+/*
+ * out[t] = residual[t] + sum_j weights[t][j] * y[row[t][j]], summed in fp32 in the order of j and rounded once.  y fp16 [y_rows][n]; out
+ * and residual (or NULL) fp16, or bf16 if out_is_bf16, and may be the same memory.  A row outside [0, y_rows) adds
+ * nothing.  n a multiple of 8, 16-byte aligned rows; strides in elements.
+ */
+int nvfp4_combine_experts(const void* y, int64_t y_row_stride, int32_t y_rows, const int32_t* row, const float* weights, int32_t tokens,
+                          int32_t top_k, int32_t n, const void* residual, int64_t residual_row_stride, void* out, int64_t out_row_stride,
+                          int32_t out_is_bf16, void* stream);
+
+/*
  * Gives back the scratch set nvfp4_gemm() assigned to `stream` on the current device (see there).
  * Call it when no GEMM of that stream is in flight any more and no graph captured on it will be
  * replayed again, e.g. before destroying the stream.

@@ -24,11 +24,14 @@ EXPORTED_SYMBOLS = (
     "nvfp4_interleave_column_blocks", "nvfp4_permute_scales", "nvfp4_gemm_allgather", "nvfp4_quantize", "nvfp4_copy_2d", "nvfp4_copy_column_blocks",
     "nvfp4_unpermute_scales", "nvfp4_compare_scale_layouts", "nvfp4_gemv_config", "nvfp4_release_stream",
     "nvfp4_gemm_epilogue", "nvfp4_plan_tile", "nvfp4_plan_segment", "nvfp4_plan_work_split", "nvfp4_plan_gemv_rows", "nvfp4_plan_tile_shape", "nvfp4_set_peer_tma_limit", "nvfp4_comm_export", "nvfp4_comm_open", "nvfp4_comm_close",
+    "nvfp4_routing_plan", "nvfp4_route", "nvfp4_plan_experts", "nvfp4_quantize_routed", "nvfp4_expert_gemm", "nvfp4_combine_experts",
 )
 COMM_HANDLE_BYTES = 64
 
-ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_SWIGLU = 0, 1, 2, 3
 OUT_FP16, OUT_NVFP4 = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+LOGITS_FP16, LOGITS_BF16, LOGITS_FP32 = 0, 1, 2
 
 
 class Nvfp4Error(RuntimeError):
@@ -66,6 +69,29 @@ class Epilogue(ctypes.Structure):
         ("out_packed_row_stride", c_int64), ("out_packed_batch_stride", c_int64),
         ("out_sf_row_stride", c_int64), ("out_sf_batch_stride", c_int64),
         ("out_sf_perm_batch_stride", c_int64), ("out_sf_perm_block_stride", c_int64),
+    ]
+
+
+class RoutingStruct(ctypes.Structure):
+    """Mirror of ``struct nvfp4_routing``."""
+    _fields_ = [("tokens", c_int32), ("top_k", c_int32), ("experts", c_int32), ("expert", c_void_p), ("row", c_void_p), ("offset", c_void_p),
+                ("plan", c_void_p)]
+
+
+class Router(ctypes.Structure):
+    """Mirror of ``struct nvfp4_router``."""
+    _fields_ = [("logits", c_void_p), ("logits_type", c_int32), ("logits_row_stride", c_int64), ("bias", c_void_p), ("scoring", c_int32),
+                ("groups", c_int32), ("top_groups", c_int32), ("group_top", c_int32), ("renormalize", c_int32), ("scale", ctypes.c_float),
+                ("weights", c_void_p)]
+
+
+class ExpertProblem(ctypes.Structure):
+    """Mirror of ``struct nvfp4_expert_problem``."""
+    _fields_ = [
+        ("a", c_void_p), ("sfa", c_void_p), ("w", c_void_p), ("sfw_perm", c_void_p), ("alpha", c_void_p), ("bias", c_void_p),
+        ("n", c_int32), ("k", c_int32), ("a_row_stride", c_int64), ("w_row_stride", c_int64), ("w_expert_stride", c_int64),
+        ("sfw_perm_expert_stride", c_int64), ("bias_expert_stride", c_int64), ("activation", c_int32), ("output", c_int32),
+        ("out_scale", ctypes.c_float), ("out", c_void_p), ("out_row_stride", c_int64), ("out_sf", c_void_p),
     ]
 
 
@@ -139,6 +165,19 @@ def load() -> ctypes.CDLL:
     lib.nvfp4_plan_tile_shape.restype = c_int
     lib.nvfp4_set_peer_tma_limit.argtypes = [c_int]
     lib.nvfp4_set_peer_tma_limit.restype = c_int
+    lib.nvfp4_routing_plan.argtypes = [c_int32] * 3 + [ctypes.POINTER(c_int32), ctypes.POINTER(c_int64), ctypes.POINTER(c_int64)]
+    lib.nvfp4_routing_plan.restype = c_int
+    lib.nvfp4_route.argtypes = [ctypes.POINTER(Router), ctypes.POINTER(RoutingStruct), c_void_p]
+    lib.nvfp4_route.restype = c_int
+    lib.nvfp4_plan_experts.argtypes = [ctypes.POINTER(RoutingStruct), c_void_p]
+    lib.nvfp4_plan_experts.restype = c_int
+    lib.nvfp4_quantize_routed.argtypes = [c_void_p, c_int32, c_int64, c_int32, ctypes.POINTER(RoutingStruct), c_void_p, c_int64, c_void_p, c_void_p]
+    lib.nvfp4_quantize_routed.restype = c_int
+    lib.nvfp4_expert_gemm.argtypes = [ctypes.POINTER(ExpertProblem), ctypes.POINTER(RoutingStruct), c_void_p]
+    lib.nvfp4_expert_gemm.restype = c_int
+    lib.nvfp4_combine_experts.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p,
+                                          c_int64, c_int32, c_void_p]
+    lib.nvfp4_combine_experts.restype = c_int
     lib.nvfp4_plan_segment.argtypes = [c_int] * 5 + [ctypes.POINTER(c_int)] * 2
     lib.nvfp4_plan_segment.restype = c_int
     lib.nvfp4_launch_count.argtypes = []

@@ -1,6 +1,6 @@
 """Ahead-of-time build of the CUDA library and the torch binding (``python -m nvfp4_gemm_b200.build``).
 
-Compiles ``csrc/nvfp4_api.cu`` for sm_100a into ``libnvfp4_b200.so`` and ``csrc/torch_binding.cpp``
+Compiles ``csrc/nvfp4_api.cu`` and ``csrc/experts_api.cu`` for sm_100a into ``libnvfp4_b200.so`` and ``csrc/torch_binding.cpp``
 (host code only) into ``_native.so`` next to this file.  nvcc cross-compiles without a GPU.  The first
 needs nvcc alone, the second g++ and the torch that it will run with.  Nothing is JIT-compiled at call
 time (the reference builds at import with ``load_inline``, s_128t.py:587-602).
@@ -15,7 +15,7 @@ import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
-SRC = PKG_DIR / "csrc" / "nvfp4_api.cu"
+SRCS = [PKG_DIR / "csrc" / "nvfp4_api.cu", PKG_DIR / "csrc" / "experts_api.cu"]
 LIB = PKG_DIR / "libnvfp4_b200.so"
 HEADER = PKG_DIR.parent / "include" / "nvfp4_b200.h"
 BINDING_SRC = PKG_DIR / "csrc" / "torch_binding.cpp"
@@ -24,7 +24,7 @@ BINDING = PKG_DIR / "_native.so"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC",
+    "--shared", "-Xcompiler", "-fPIC", "--threads", "2",
     "-cudart", "static",
 ]
 
@@ -37,7 +37,7 @@ def find_nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return [SRC, *sorted((PKG_DIR / "csrc").glob("*.cuh")), HEADER]
+    return [*SRCS, PKG_DIR / "csrc" / "api_internal.h", *sorted((PKG_DIR / "csrc").glob("*.cuh")), HEADER]
 
 
 def _newer(target: Path, inputs: list[Path]) -> bool:
@@ -109,7 +109,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     """Builds what is out of date.  The C library needs nvcc alone; where the binding cannot be built, a
     caller of the C library is told so and gets it all the same (``_lib.native()`` refuses to go on without)."""
     if force or not _newer(LIB, sources()):
-        _replace(LIB, [find_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, str(SRC)], verbose)
+        _replace(LIB, [find_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, *map(str, SRCS)], verbose)
     why = why_no_binding()
     if why is not None:
         print(f"{BINDING.name} (calls on torch tensors) is not built: {why}", file=sys.stderr)

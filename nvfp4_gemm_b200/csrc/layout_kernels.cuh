@@ -186,47 +186,6 @@ struct QuantizeParams {
     long long x_row_stride, packed_row_stride, sf_plain_row_stride;   // bytes
 };
 template <bool kWide>
-__device__ __forceinline__ void load_block16(const uint8_t* src, uint32_t (&w)[8]) {
-    if (kWide) {
-        asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(src));
-    } else {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src)), b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
-    }
-}
-// Sixteen fp16 / bf16 values -> eight bytes of codes and the scale byte.
-template <bool BF16>
-__device__ __forceinline__ uint32_t quantize_words(const uint32_t (&w)[8], uint32_t (&codes)[2]) {
-    float v[16], amax;
-    if (BF16) {
-        __nv_bfloat162 top = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
-        const uint32_t t = *reinterpret_cast<const uint32_t*>(&top);
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(__uint_as_float(t << 16)), "f"(__uint_as_float(t & 0xffff0000u)));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[2 * j] = __uint_as_float(w[j] << 16);
-            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    } else {
-        __half2 top = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[j])));
-        const float2 t = __half22float2(top);
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(t.x), "f"(t.y));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-        }
-    }
-    return quantize_block16(v, amax, codes);
-}
-template <bool kWide>
 __device__ __forceinline__ void store_scale_word(uint8_t* at, uint32_t w) {
     if (kWide) {
         *reinterpret_cast<uint32_t*>(at) = w;

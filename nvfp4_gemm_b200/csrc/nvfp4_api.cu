@@ -4,24 +4,21 @@
 #include "../../include/nvfp4_b200.h"
 
 #include <algorithm>
-#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
-#include <cstring>
 #include <mutex>
-#include <string>
 
+#include "api_internal.h"
 #include "gemm_decode_sm100.cuh"
 #include "gemm_sm100.cuh"
 #include "gemv_sm100.cuh"
 #include "layout_kernels.cuh"
 
-namespace {
+namespace nvfp4 {
+namespace host {
 
-using namespace nvfp4;
-
-thread_local std::string t_error;
+static thread_local std::string t_error;
 thread_local const char* t_last_kernel = "";
 std::atomic<uint64_t> g_launches{0};
 std::atomic<uint64_t> g_timeout_ns{1000000000ull};
@@ -36,26 +33,9 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define CUDA_TRY(expr)                                                                             \
-    do {                                                                                           \
-        cudaError_t e__ = (expr);                                                                  \
-        if (e__ != cudaSuccess) return fail(NVFP4_ERR_CUDA, "%s failed: %s", #expr, cudaGetErrorString(e__)); \
-    } while (0)
-
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// What a tensor map is encoded from.
-struct MapKey {
-    const void* ptr;
-    uint64_t dims[4];
-    uint64_t strides[3];
-    uint32_t box[4];
-    int dtype;
-    int rank;
-    int swizzle;
-};
 
 constexpr int kMaxCtas = 160;                                          // persistent CTAs (one per SM; a B200 has 148)
 constexpr size_t kSlotBytes = static_cast<size_t>(kBM) * 256 * sizeof(float);  // one 128 x 256 fp32 partial tile
@@ -66,30 +46,12 @@ constexpr size_t kScratchBytes = kMaxCtas * 2 * kSlotBytes;             // head 
 // inside a graph capture).  A set stays with its stream until nvfp4_release_stream(); when all
 // are taken, sets of streams that have gone idle are taken back -- except sets that were used
 // while their stream was being captured: a graph may replay those launches at any later time.
-constexpr int kStreamSets = 8;
 
-struct DeviceCtx {
-    int device = -1;
-    int num_sms = 0;
-    bool sm100 = false;
-    float* scratch = nullptr;    // kStreamSets sets of partial-tile slots
-    int* counters = nullptr;     // kStreamSets sets of tile counters
-    cudaStream_t set_stream[kStreamSets] = {};
-    bool set_used[kStreamSets] = {};
-    bool set_in_graph[kStreamSets] = {};   // a launch with this set was recorded into a CUDA graph
-    int* status_host = nullptr;
-    int* status_dev = nullptr;
-    size_t scratch_bytes = 0;
-    std::atomic<bool> scratch_ready{false};   // scratch and counters are allocated and cleared
-    int max_pairs = -1;  // CTA pairs that can be co-resident (cluster occupancy), queried once
-    std::atomic<bool> smem_attr_set[52] = {};   // by kernel variant: 0..23 the tiled kernels, 24.. the decode kernels
-};
+static std::mutex g_mutex;
+static std::atomic<DeviceCtx*> g_ctx[64];
+static std::atomic<EncodeTiledFn> g_encode{nullptr};
 
-std::mutex g_mutex;
-std::atomic<DeviceCtx*> g_ctx[64];
-std::atomic<EncodeTiledFn> g_encode{nullptr};
-
-int find_encode(EncodeTiledFn* out) {
+static int find_encode(EncodeTiledFn* out) {
     *out = g_encode.load(std::memory_order_acquire);
     if (*out) return NVFP4_OK;
     void* fn = nullptr;
@@ -125,7 +87,7 @@ int get_ctx(DeviceCtx** out) {
     return NVFP4_OK;
 }
 
-int ensure_scratch(DeviceCtx* c) {
+static int ensure_scratch(DeviceCtx* c) {
     if (c->scratch_ready.load(std::memory_order_acquire)) return NVFP4_OK;
     std::lock_guard<std::mutex> lock(g_mutex);
     if (c->scratch_ready.load()) return NVFP4_OK;
@@ -141,7 +103,7 @@ int ensure_scratch(DeviceCtx* c) {
 }
 
 // The scratch set of `stream` on this device.
-int scratch_set_for(DeviceCtx* c, cudaStream_t stream, int* set) {
+static int scratch_set_for(DeviceCtx* c, cudaStream_t stream, int* set) {
     std::lock_guard<std::mutex> lock(g_mutex);
     for (int i = 0; i < kStreamSets; ++i)
         if (c->set_used[i] && c->set_stream[i] == stream) {
@@ -233,7 +195,13 @@ MapKey make_sf_key(const void* ptr, int rows, int k, int l, uint64_t batch_strid
     return key;
 }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+}  // namespace host
+}  // namespace nvfp4
+
+namespace {
+
+using namespace nvfp4;
+using namespace nvfp4::host;
 
 // Whole tiles per worker, or an even split of all (tile, k-tile) units with shared tiles summed
 // through scratch?  In k-tiles of run time: whole tiles cost waves x k_tiles; the even split costs

@@ -339,6 +339,22 @@ __device__ __forceinline__ void tc_ld_32cols(uint32_t taddr, uint32_t (&r)[32]) 
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
+// 32 consecutive fp32 columns of 16 TMEM lanes, in the fragment order of a matrix instruction's
+// result: r[4 * c + {0, 1}] = lane thread/4, columns 8 * c + 2 * (thread % 4) + {0, 1}; r[4 * c + {2, 3}] the
+// same columns of lane thread/4 + 8.  The address names the first lane (a multiple of 16).
+__device__ __forceinline__ void tc_ld_16lanes_32cols(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values, turned round on their way to shared memory: this thread holds
+// row lane/4, columns 2 * (lane % 4) + {0, 1} of each; 16-byte row r of matrix m is written to the address that lane 8 * m + r gives
+// and holds column r of it.
+__device__ __forceinline__ void st_matrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ------------------------------------------------------------- descriptors

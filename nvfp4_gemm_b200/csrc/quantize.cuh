@@ -1,6 +1,7 @@
 // The NVFP4 rounding rule, shared by the stand-alone quantiser (layout_kernels.cuh) and the GEMM's
 // re-quantising epilogue (gemm_sm100.cuh) so that the two produce the same bytes.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -103,4 +104,46 @@ __device__ __forceinline__ uint8_t quantize_block16(float (&v)[16], uint32_t (&o
     return quantize_block16(v, amax, out);
 }
 
+// Sixteen fp16 / bf16 values of a row, 32 bytes; kWide: src is 32-byte aligned (otherwise 16).
+template <bool kWide>
+__device__ __forceinline__ void load_block16(const uint8_t* src, uint32_t (&w)[8]) {
+    if (kWide) {
+        asm volatile("ld.global.L1::no_allocate.L2::evict_first.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(src));
+    } else {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src)), b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
+        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+        w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+    }
+}
+// Sixteen fp16 / bf16 values -> eight bytes of codes and the scale byte.
+template <bool BF16>
+__device__ __forceinline__ uint32_t quantize_words(const uint32_t (&w)[8], uint32_t (&codes)[2]) {
+    float v[16], amax;
+    if (BF16) {
+        __nv_bfloat162 top = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])));
+        const uint32_t t = *reinterpret_cast<const uint32_t*>(&top);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(__uint_as_float(t << 16)), "f"(__uint_as_float(t & 0xffff0000u)));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+    } else {
+        __half2 top = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[j])));
+        const float2 t = __half22float2(top);
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(amax) : "f"(t.x), "f"(t.y));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
+    }
+    return quantize_block16(v, amax, codes);
+}
 }  // namespace nvfp4

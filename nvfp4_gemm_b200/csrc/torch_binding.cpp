@@ -10,6 +10,7 @@
 // 3.75 us a pass; a first call on new tensors 28.5 -> 17.6 us, waited for).
 #include <Python.h>
 
+#include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -17,6 +18,7 @@
 
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 
 #include "../../include/nvfp4_b200.h"
 
@@ -130,7 +132,7 @@ nvfp4_problem make_problem(const Operands& o) {
 
 // Calls f(stream) with the tensors' device current, on torch's current stream of that device and
 // without the interpreter lock (a launch waits when the queue of the device is full).  Only f, which
-// answers with a status, runs unlocked: the guard and the stream throw where CUDA reports an error, and
+// answers with a status and throws nothing, runs unlocked: the guard and the stream throw where CUDA reports an error, and
 // an exception that left with the lock released would be turned into a Python one without a thread state.
 template <class F>
 int on_current_stream(const at::Tensor& a, F f) {
@@ -233,6 +235,312 @@ PyObject* py_gemm_epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     });
 }
 
+// ------------------------------------------------------------------------------------- mixture of experts
+// Each call checks its tensors, allocates its results and answers with them, or with the status (an int) where the C ABI refused.
+
+const at::Tensor& tensor_arg(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "%s must be a tensor, got %s", name, Py_TYPE(o)->tp_name);
+        throw PythonError{};
+    }
+    return THPVariable_Unpack(o);
+}
+
+[[noreturn]] void raise_value(const char* fmt, const char* name) {
+    PyErr_Format(PyExc_ValueError, fmt, name);
+    throw PythonError{};
+}
+
+// `t` lives on the device of `on` (a CUDA device).
+void same_device(const at::Tensor& t, const at::Tensor& on, const char* name) {
+    if (!on.is_cuda() || !t.is_cuda()) raise(PyExc_ValueError, "the experts' operators need CUDA tensors (there is no CPU fallback)");
+    if (t.device() != on.device()) raise_value("%s is on another device than the first tensor", name);
+}
+
+int32_t size_arg(int64_t v, const char* name) {
+    if (v > INT32_MAX) raise_value("%s does not fit 32 bits", name);
+    return static_cast<int32_t>(v);
+}
+
+// A [rows, columns] tensor whose rows are contiguous.
+void rows_of(const at::Tensor& t, const char* name) {
+    if (t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1)) raise_value("%s must have two dimensions, the second contiguous", name);
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// What a call makes itself, on the device of `on`.
+at::Tensor fresh(const at::Tensor& on, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, on.options().dtype(type)); }
+
+PyObject* status_object(int rc) { return PyLong_FromLong(rc); }
+
+PyObject* pack(std::initializer_list<at::Tensor> tensors) {
+    PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+    if (!out) throw PythonError{};
+    Py_ssize_t i = 0;
+    for (const at::Tensor& t : tensors) {
+        PyObject* o = THPVariable_Wrap(t);
+        if (!o) {
+            Py_DECREF(out);
+            throw PythonError{};
+        }
+        PyTuple_SET_ITEM(out, i++, o);
+    }
+    return out;
+}
+
+// The routing that belongs to choices of this shape, with new memory for what is not given.
+struct Routing {
+    nvfp4_routing r;
+    int64_t sf_rows = 0;
+    at::Tensor row, offset, plan;
+    int status;
+    // new rows, offsets and plan for [tokens, top_k] choices
+    Routing(const at::Tensor& on, int64_t tokens, int64_t top_k, int64_t experts) {
+        int64_t plan_bytes = 0;
+        status = size(tokens, top_k, experts, &plan_bytes);
+        if (status) return;
+        row = fresh(on, {tokens, top_k}, at::kInt);
+        offset = fresh(on, {experts + 1}, at::kInt);
+        plan = fresh(on, {plan_bytes / 4}, at::kInt);
+        r.row = row.data_ptr<int32_t>();
+        r.offset = offset.data_ptr<int32_t>();
+        r.plan = plan.data_ptr();
+    }
+    // the rows and plan of an earlier call
+    Routing(const at::Tensor& on, PyObject* rows, PyObject* plan_o, PyObject* experts) {
+        row = tensor_arg(rows, "rows");
+        plan = tensor_arg(plan_o, "plan");
+        same_device(row, on, "rows");
+        same_device(plan, on, "plan");
+        if (row.dim() != 2 || row.scalar_type() != at::kInt || !row.is_contiguous() || plan.scalar_type() != at::kInt || !plan.is_contiguous())
+            raise(PyExc_ValueError, "rows and plan must be what route() or plan() returned (contiguous int32)");
+        int64_t plan_bytes = 0;
+        const long long e = PyLong_AsLongLong(experts);
+        if (e == -1 && PyErr_Occurred()) throw PythonError{};
+        status = size(row.size(0), row.size(1), e, &plan_bytes);
+        if (status) return;
+        if (plan.numel() * 4 != plan_bytes) raise(PyExc_ValueError, "plan does not belong to rows of this shape and to this number of experts");
+        r.row = row.data_ptr<int32_t>();
+        r.plan = plan.data_ptr();
+    }
+
+private:
+    int size(int64_t tokens, int64_t top_k, int64_t experts, int64_t* plan_bytes) {
+        std::memset(&r, 0, sizeof(r));
+        r.tokens = size_arg(tokens, "the number of tokens");
+        r.top_k = size_arg(top_k, "top_k");
+        r.experts = size_arg(experts, "the number of experts");
+        return nvfp4_routing_plan(r.tokens, r.top_k, r.experts, nullptr, plan_bytes, &sf_rows);
+    }
+};
+
+double float_arg(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PythonError{};
+    return v;
+}
+
+// route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan)
+PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 9) raise(PyExc_TypeError, "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale)");
+        const at::Tensor& logits = tensor_arg(args[0], "logits");
+        same_device(logits, logits, "logits");
+        rows_of(logits, "logits");
+        nvfp4_router o;
+        std::memset(&o, 0, sizeof(o));
+        if (logits.scalar_type() == at::kFloat) o.logits_type = NVFP4_LOGITS_FP32;
+        else if (logits.scalar_type() == at::kBFloat16) o.logits_type = NVFP4_LOGITS_BF16;
+        else if (logits.scalar_type() == at::kHalf) o.logits_type = NVFP4_LOGITS_FP16;
+        else raise(PyExc_ValueError, "logits must be fp16, bf16 or fp32");
+        const int top_k = int_arg(args[1]);
+        o.scoring = int_arg(args[2]);
+        if (const at::Tensor* bias = tensor_or_none(args[3])) {
+            same_device(*bias, logits, "bias");
+            if (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != logits.size(1) || !bias->is_contiguous())
+                raise(PyExc_ValueError, "bias must be a contiguous fp32 vector with an entry per expert");
+            o.bias = bias->data_ptr<float>();
+        }
+        o.groups = int_arg(args[4]);
+        o.top_groups = int_arg(args[5]);
+        o.group_top = int_arg(args[6]);
+        o.renormalize = int_arg(args[7]);
+        o.scale = static_cast<float>(float_arg(args[8]));
+        const c10::cuda::CUDAGuard guard(logits.device());
+        Routing routing(logits, logits.size(0), top_k, logits.size(1));
+        if (routing.status) return status_object(routing.status);
+        const at::Tensor experts = fresh(logits, {logits.size(0), top_k}, at::kInt), weights = fresh(logits, {logits.size(0), top_k}, at::kFloat);
+        routing.r.expert = experts.data_ptr<int32_t>();
+        o.logits = logits.data_ptr();
+        o.logits_row_stride = row_stride(logits);
+        o.weights = weights.data_ptr<float>();
+        const int rc = on_current_stream(logits, [&](void* stream) { return nvfp4_route(&o, &routing.r, stream); });
+        return rc ? status_object(rc) : pack({experts, weights, routing.row, routing.offset, routing.plan});
+    });
+}
+
+// plan(experts, number of experts) -> (rows, offsets, plan)
+PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 2) raise(PyExc_TypeError, "plan(experts, number of experts)");
+        const at::Tensor& experts = tensor_arg(args[0], "experts");
+        same_device(experts, experts, "experts");
+        if (experts.dim() != 2 || experts.scalar_type() != at::kInt || !experts.is_contiguous())
+            raise(PyExc_ValueError, "experts must be a contiguous int32 tensor [tokens, top_k]");
+        const c10::cuda::CUDAGuard guard(experts.device());
+        Routing routing(experts, experts.size(0), experts.size(1), int_arg(args[1]));
+        if (routing.status) return status_object(routing.status);
+        routing.r.expert = experts.data_ptr<int32_t>();
+        const int rc = on_current_stream(experts, [&](void* stream) { return nvfp4_plan_experts(&routing.r, stream); });
+        return rc ? status_object(rc) : pack({routing.row, routing.offset, routing.plan});
+    });
+}
+
+// quantize_routed(x, rows, plan, number of experts) -> (packed, sf)
+PyObject* py_quantize_routed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 4) raise(PyExc_TypeError, "quantize_routed(x, rows, plan, number of experts)");
+        const at::Tensor& x = tensor_arg(args[0], "x");
+        same_device(x, x, "x");
+        rows_of(x, "x");
+        if (x.scalar_type() != at::kHalf && x.scalar_type() != at::kBFloat16) raise(PyExc_ValueError, "x must be fp16 or bf16");
+        const c10::cuda::CUDAGuard guard(x.device());
+        Routing routing(x, args[1], args[2], args[3]);
+        if (routing.status) return status_object(routing.status);
+        if (routing.r.tokens != x.size(0)) raise(PyExc_ValueError, "x must have a row per token of the routing");
+        const int64_t k = size_arg(x.size(1), "the width of x");
+        const at::Tensor packed = fresh(x, {routing.row.numel(), k / 2}, at::kFloat4_e2m1fn_x2);
+        const at::Tensor sf = fresh(x, {routing.sf_rows * (k / 16)}, at::kFloat8_e4m3fn);
+        const void* const src = x.data_ptr();
+        void *const codes = packed.data_ptr(), *const scales = sf.data_ptr();
+        const bool bf16 = x.scalar_type() == at::kBFloat16;
+        const int64_t stride = row_stride(x);
+        const int rc = on_current_stream(
+            x, [&](void* stream) { return nvfp4_quantize_routed(src, bf16, stride, static_cast<int32_t>(k), &routing.r, codes, k / 2, scales, stream); });
+        return rc ? status_object(rc) : pack({packed, sf});
+    });
+}
+
+// expert_gemm(packed, sf, rows, plan, number of experts, w, w_sf_permuted, alpha, bias, activation, out_scale, nvfp4_out, out)
+//   -> (y,) or (packed, sf)
+PyObject* py_expert_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 13)
+            raise(PyExc_TypeError, "expert_gemm(packed, sf, rows, plan, number of experts, w, w_sf_permuted, alpha, bias, activation, out_scale, nvfp4_out, out)");
+        const at::Tensor &a = tensor_arg(args[0], "packed"), &sfa = tensor_arg(args[1], "sf");
+        const at::Tensor &w = tensor_arg(args[5], "w"), &sfw = tensor_arg(args[6], "w_sf_permuted");
+        same_device(a, a, "packed");
+        same_device(sfa, a, "sf");
+        same_device(w, a, "w");
+        same_device(sfw, a, "w_sf_permuted");
+        const c10::cuda::CUDAGuard guard(a.device());
+        Routing routing(a, args[2], args[3], args[4]);
+        if (routing.status) return status_object(routing.status);
+        const int64_t experts = routing.r.experts, rows = routing.row.numel();
+        rows_of(a, "packed");
+        if (w.dim() != 3 || w.stride(1) != 1) raise(PyExc_ValueError, "w must be [n, k / 2, experts] with the second dimension contiguous");
+        const int64_t n = w.size(0), kb = w.size(1), rest_n = (n + 127) / 128, rest_k = kb / 32;
+        if (a.element_size() != 1 || w.element_size() != 1 || sfa.element_size() != 1 || sfw.element_size() != 1)
+            raise(PyExc_ValueError, "expected packed fp4 (1 byte per 2 values) and 1-byte scales");
+        if (a.size(0) != rows || a.size(1) != kb || w.size(2) != experts) raise(PyExc_ValueError, "packed, w and the routing disagree on rows, k or experts");
+        if (!sfa.is_contiguous() || sfa.numel() != routing.sf_rows * (kb / 8)) raise(PyExc_ValueError, "sf is not the scales of a routed operand of this routing and k");
+        const int64_t sizes[6] = {32, 4, rest_n, 4, rest_k, experts}, strides[5] = {16, 4, rest_k * 512, 1, 512};
+        bool fits = sfw.dim() == 6;
+        for (int i = 0; fits && i < 6; ++i) fits = sfw.size(i) == sizes[i] && (i == 5 || sizes[i] == 1 || sfw.stride(i) == strides[i]);
+        if (!fits) raise(PyExc_ValueError, "w_sf_permuted must be [32, 4, n / 128, 4, k / 64, experts] in 512-byte atoms");
+        nvfp4_expert_problem p;
+        std::memset(&p, 0, sizeof(p));
+        if (const at::Tensor* t = tensor_or_none(args[7])) {
+            same_device(*t, a, "alpha");
+            if (t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != experts || !t->is_contiguous())
+                raise(PyExc_ValueError, "alpha must be a contiguous fp32 vector with an entry per expert");
+            p.alpha = t->data_ptr<float>();
+        }
+        if (const at::Tensor* t = tensor_or_none(args[8])) {
+            same_device(*t, a, "bias");
+            if (t->scalar_type() != at::kHalf || t->dim() != 2 || t->size(0) != experts || t->size(1) != n || (n > 1 && t->stride(1) != 1))
+                raise(PyExc_ValueError, "bias must be fp16 [experts, n] with contiguous rows");
+            p.bias = t->data_ptr();
+            p.bias_expert_stride = t->size(0) > 1 ? t->stride(0) : n;
+        }
+        p.activation = int_arg(args[9]);
+        p.out_scale = static_cast<float>(float_arg(args[10]));
+        const bool to_nvfp4 = int_arg(args[11]) != 0;
+        const int64_t n_out = p.activation == NVFP4_ACT_SWIGLU ? n / 2 : n;
+        p.a = a.data_ptr();
+        p.sfa = sfa.data_ptr();
+        p.w = w.data_ptr();
+        p.sfw_perm = sfw.data_ptr();
+        p.n = size_arg(n, "n");
+        p.k = size_arg(2 * kb, "k");
+        p.a_row_stride = rows > 1 ? a.stride(0) : kb;
+        p.w_row_stride = w.stride(0);
+        p.w_expert_stride = w.stride(2);
+        p.sfw_perm_expert_stride = sfw.stride(5);
+        at::Tensor out, out_sf;
+        if (to_nvfp4) {
+            if (args[12] != Py_None) raise(PyExc_ValueError, "out is for the fp16 result");
+            out = fresh(a, {rows, n_out / 2}, at::kFloat4_e2m1fn_x2);
+            out_sf = fresh(a, {routing.sf_rows * (n_out / 16)}, at::kFloat8_e4m3fn);
+            p.output = NVFP4_OUT_NVFP4;
+            p.out_row_stride = n_out / 2;
+            p.out_sf = out_sf.data_ptr();
+        } else if (const at::Tensor* t = tensor_or_none(args[12])) {
+            same_device(*t, a, "out");
+            rows_of(*t, "out");
+            if (t->scalar_type() != at::kHalf || t->size(0) != rows || t->size(1) != n_out) raise(PyExc_ValueError, "out must be fp16 [tokens * top_k, columns]");
+            out = *t;
+            p.out_row_stride = row_stride(out);
+        } else {
+            out = fresh(a, {rows, n_out}, at::kHalf);
+            p.out_row_stride = n_out;
+        }
+        p.out = out.data_ptr();
+        const int rc = on_current_stream(a, [&](void* stream) { return nvfp4_expert_gemm(&p, &routing.r, stream); });
+        if (rc) return status_object(rc);
+        return to_nvfp4 ? pack({out, out_sf}) : pack({out});
+    });
+}
+
+// combine(y, rows, weights, residual, out, bf16) -> (out,)
+PyObject* py_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject* {
+        if (nargs != 6) raise(PyExc_TypeError, "combine(y, rows, weights, residual, out, bf16)");
+        const at::Tensor &y = tensor_arg(args[0], "y"), &rows = tensor_arg(args[1], "rows"), &weights = tensor_arg(args[2], "weights");
+        same_device(y, y, "y");
+        same_device(rows, y, "rows");
+        same_device(weights, y, "weights");
+        rows_of(y, "y");
+        if (y.scalar_type() != at::kHalf) raise(PyExc_ValueError, "y must be fp16");
+        if (rows.dim() != 2 || rows.scalar_type() != at::kInt || !rows.is_contiguous()) raise(PyExc_ValueError, "rows must be contiguous int32 [tokens, top_k]");
+        if (weights.sizes() != rows.sizes() || weights.scalar_type() != at::kFloat || !weights.is_contiguous())
+            raise(PyExc_ValueError, "weights must be contiguous fp32 of the shape of rows");
+        const int64_t tokens = rows.size(0), n = y.size(1);
+        const at::ScalarType type = int_arg(args[5]) ? at::kBFloat16 : at::kHalf;
+        const at::Tensor* residual = tensor_or_none(args[3]);
+        const at::Tensor* given = tensor_or_none(args[4]);
+        const char* const names[2] = {"residual", "out"};
+        for (int i = 0; i < 2; ++i)
+            if (const at::Tensor* t = i ? given : residual) {
+                same_device(*t, y, names[i]);
+                rows_of(*t, names[i]);
+                if (t->size(0) != tokens || t->size(1) != n || t->scalar_type() != type) raise_value("%s must be [tokens, n] of the output's type", names[i]);
+            }
+        const c10::cuda::CUDAGuard guard(y.device());
+        const at::Tensor out = given ? *given : fresh(y, {tokens, n}, type);
+        const int32_t y_rows = size_arg(y.size(0), "y"), t = size_arg(tokens, "the number of tokens"), top_k = size_arg(rows.size(1), "top_k"), cols = size_arg(n, "n");
+        const void *const src = y.data_ptr(), *const add = residual ? residual->data_ptr() : nullptr;
+        const int32_t* const row = rows.data_ptr<int32_t>();
+        const float* const weight = weights.data_ptr<float>();
+        void* const dst = out.data_ptr();
+        const int64_t y_stride = row_stride(y), add_stride = residual ? row_stride(*residual) : 0, out_stride = row_stride(out);
+        const int rc = on_current_stream(y, [&](void* stream) {
+            return nvfp4_combine_experts(src, y_stride, y_rows, row, weight, t, top_k, cols, add, add_stride, dst, out_stride, type == at::kBFloat16, stream);
+        });
+        return rc ? status_object(rc) : pack({out});
+    });
+}
+
 // Read from the file by nvfp4_gemm_b200/build.py: the types of torch and Python that this code has the layouts of.
 [[gnu::used]] const char built_for[] = "nvfp4_native built for: " NVFP4_BUILT_FOR;
 
@@ -241,6 +549,14 @@ PyMethodDef methods[] = {
     {"fill_problem", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_fill_problem)), METH_FASTCALL, "fill_problem(data, address)"},
     {"gemm_epilogue", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_gemm_epilogue)), METH_FASTCALL,
      "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k) -> status"},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_route)), METH_FASTCALL,
+     "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan) or status"},
+    {"plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_plan)), METH_FASTCALL, "plan(experts, number of experts) -> (rows, offsets, plan) or status"},
+    {"quantize_routed", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_quantize_routed)), METH_FASTCALL,
+     "quantize_routed(x, rows, plan, number of experts) -> (packed, sf) or status"},
+    {"expert_gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_expert_gemm)), METH_FASTCALL,
+     "expert_gemm(packed, sf, rows, plan, number of experts, w, w_sf_permuted, alpha, bias, activation, out_scale, nvfp4_out, out) -> (y,), (packed, sf) or status"},
+    {"combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_combine)), METH_FASTCALL, "combine(y, rows, weights, residual, out, bf16) -> (out,) or status"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "torch tensors to the C ABI of libnvfp4_b200", -1, methods, nullptr, nullptr, nullptr, nullptr};
