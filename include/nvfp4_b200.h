@@ -122,6 +122,16 @@ typedef struct nvfp4_epilogue {
 int nvfp4_gemm_epilogue(const nvfp4_problem* problem, const nvfp4_gemm_config* cfg, const nvfp4_epilogue* epilogue, void* stream);
 
 /*
+ * nvfp4_gemm_epilogue() with a residual: out = act(acc + bias[column]) + residual[l][m][column], added in fp32 ahead of the one
+ * rounding to fp16 (which the NVFP4 form quantises): the step that closes a layer's output projection.  residual: fp16,
+ * 16-byte aligned, strides in elements, multiples of 8; a stride of 0 repeats rows or batches.  It may be the memory of
+ * problem->c itself (with c's strides), or lie apart from what is written.  epilogue may be NULL (no bias, no
+ * activation, fp16).  The reference has no counterpart.
+ */
+int nvfp4_gemm_residual(const nvfp4_problem* problem, const nvfp4_gemm_config* cfg, const nvfp4_epilogue* epilogue, const void* residual,
+                        int64_t residual_row_stride, int64_t residual_batch_stride, void* stream);
+
+/*
  * CUDA-core GEMV for n == 1.  Replaces cuda_nvfp4_gemv(A, B, C, SFA, SFB) of
  * old_files/1.py:610-673.  Requires k % 64 == 0 (task_gemv.yml:24) and 32-byte aligned rows.
  */

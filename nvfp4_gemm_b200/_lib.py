@@ -25,6 +25,7 @@ EXPORTED_SYMBOLS = (
     "nvfp4_unpermute_scales", "nvfp4_compare_scale_layouts", "nvfp4_gemv_config", "nvfp4_release_stream",
     "nvfp4_gemm_epilogue", "nvfp4_plan_tile", "nvfp4_plan_segment", "nvfp4_plan_work_split", "nvfp4_plan_gemv_rows", "nvfp4_plan_tile_shape", "nvfp4_set_peer_tma_limit", "nvfp4_comm_export", "nvfp4_comm_open", "nvfp4_comm_close",
     "nvfp4_routing_plan", "nvfp4_route", "nvfp4_plan_experts", "nvfp4_quantize_routed", "nvfp4_expert_gemm", "nvfp4_combine_experts",
+    "nvfp4_gemm_residual",
 )
 COMM_HANDLE_BYTES = 64
 
@@ -111,6 +112,8 @@ def load() -> ctypes.CDLL:
     lib.nvfp4_gemm.restype = c_int
     lib.nvfp4_gemm_epilogue.argtypes = [ctypes.POINTER(Problem), ctypes.POINTER(GemmConfig), ctypes.POINTER(Epilogue), c_void_p]
     lib.nvfp4_gemm_epilogue.restype = c_int
+    lib.nvfp4_gemm_residual.argtypes = [ctypes.POINTER(Problem), ctypes.POINTER(GemmConfig), ctypes.POINTER(Epilogue), c_void_p, c_int64, c_int64, c_void_p]
+    lib.nvfp4_gemm_residual.restype = c_int
     lib.nvfp4_gemm_static_scratch.argtypes = [ctypes.POINTER(Problem), c_int, c_void_p]
     lib.nvfp4_gemm_static_scratch.restype = c_int
     lib.nvfp4_interleave_column_blocks.argtypes = [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int64, c_void_p]

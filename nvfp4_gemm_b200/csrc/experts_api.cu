@@ -318,10 +318,10 @@ int nvfp4_expert_gemm(const nvfp4_expert_problem* p, const nvfp4_routing* r, voi
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     if (s.tile_tokens == kTileFew) {
         g.tiles_n = p->n / kBM;
-        return launch_expert_gemm<1, kTileFew, 4, 4, 2>(c, 50, g, s.max_tiles, stream, "expert_gemm_t32");
+        return launch_expert_gemm<1, kTileFew, 4, 4, 2>(c, 72, g, s.max_tiles, stream, "expert_gemm_t32");
     }
     g.tiles_n = (p->n + 2 * kBM - 1) / (2 * kBM);
-    return launch_expert_gemm<2, kTileMany, 5, 8, 1>(c, 51, g, s.max_tiles, stream, "expert_gemm_2cta_t256");
+    return launch_expert_gemm<2, kTileMany, 5, 8, 1>(c, 73, g, s.max_tiles, stream, "expert_gemm_2cta_t256");
 }
 
 int nvfp4_combine_experts(const void* y, int64_t y_row_stride, int32_t y_rows, const int32_t* row, const float* weights, int32_t tokens, int32_t top_k,

@@ -52,6 +52,10 @@ constexpr int kSfaColOverlap = 384, kSfbColOverlap = 416;
 
 enum Activation : int { kActNone = 0, kActRelu = 1, kActSilu = 2 };
 
+// What a kernel does with a finished accumulator: fp16 as it is; bias, activation and NVFP4 output; and the same
+// with a residual.  (A form of its own: the loads and the larger code are not for those that have none.)
+constexpr int kEpiPlain = 0, kEpiExtended = 1, kEpiResidual = 2;
+
 enum GemmStatus : int {
     kStatusOk = 0,
     kStatusWaitTimeout = 1,  // a bounded mbarrier wait ran out
@@ -78,6 +82,8 @@ struct GemmParams {
     // as fp16 to c, or re-quantised to NVFP4 (packed e2m1 + one e4m3 scale per 16 columns of a row,
     // the operand format of a following GEMM whose K is this GEMM's N).
     const __half* bias;          // [N] or null
+    const __half* residual;      // (EPI_EX == kEpiResidual) [L][M][N], added behind the activation
+    long long residual_row_stride, residual_batch_stride;       // elements
     int activation;              // kActNone / kActRelu / kActSilu
     int out_nvfp4;               // 0: fp16 to c; 1: packed + scales
     uint8_t* out_packed;         // [L][M][N/2]
@@ -281,6 +287,28 @@ __device__ __forceinline__ void bias_act16(const GemmParams& p, int gcol, float*
     }
 }
 
+// The residual's COLS columns (a multiple of 8) of one row from gcol on: requested together, ahead of the arithmetic
+// that they are added behind.
+template <int COLS>
+__device__ __forceinline__ void load_residual(const GemmParams& p, int l, long long row, int gcol, uint4 (&r)[COLS / 8]) {
+    const __half* src = p.residual + l * p.residual_batch_stride + row * p.residual_row_stride + gcol;
+#pragma unroll
+    for (int j = 0; j < COLS / 8; ++j) r[j] = *reinterpret_cast<const uint4*>(src + 8 * j);
+}
+// s[0..15] += sixteen fp16 of the residual
+__device__ __forceinline__ void add_residual16(const uint4 (&r)[2], float* s) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            s[8 * j + 2 * e] = __fadd_rn(s[8 * j + 2 * e], f.x);
+            s[8 * j + 2 * e + 1] = __fadd_rn(s[8 * j + 2 * e + 1], f.y);
+        }
+    }
+}
+
 // At the end of a CTA whose wait ran out: longer than a copy into shared memory that is on its way can take.
 __device__ __forceinline__ void let_copies_land() {
     constexpr long long kCycles = 40000;          // 20 us at the highest clock; a copy takes one or two
@@ -324,7 +352,7 @@ __device__ __forceinline__ void leave_cluster(bool gave_up) {
     }
 }
 
-template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int KS = 1, bool EPI_EX = false, int EPI_WARPS = 0>
+template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int KS = 1, int EPI_EX = kEpiPlain, int EPI_WARPS = 0>
 __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS>::kThreads, 1) gemm_nvfp4_kernel(const __grid_constant__ GemmParams p) {
     static_assert(!(EPI_EX && TMA_STORE), "the extended epilogue writes with plain stores");
     using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS>;
@@ -663,6 +691,8 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     // once.  Codes and scales of the NVFP4 form are collected and stored together: 64
                     // columns are 32 bytes of codes (one full sector) and the four scales of one unit of either layout.
                     const int gcol = nb * BN + c0;
+                    [[maybe_unused]] uint4 res[EPI_EX == kEpiResidual ? kCols / 8 : 2];
+                    if constexpr (EPI_EX == kEpiResidual) load_residual<kCols>(p, l, row, gcol, res);
                     uint32_t q[kCols / 8];
                     uint32_t sf = 0u;
 #pragma unroll
@@ -670,6 +700,12 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
 #pragma unroll 1
                     for (int h = 0; h < kCols; h += 16) {
                         bias_act16(p, gcol + h, s);
+                        if constexpr (EPI_EX == kEpiResidual) {
+                            const uint4 now[2] = {res[0], res[1]};
+                            add_residual16(now, s);
+#pragma unroll
+                            for (int j = 0; j + 2 < kCols / 8; ++j) res[j] = res[j + 2];
+                        }
                         if (!p.out_nvfp4) {
                             store8(c0 + h, pack8_fp16(&s[0]));
                             store8(c0 + h + 8, pack8_fp16(&s[8]));

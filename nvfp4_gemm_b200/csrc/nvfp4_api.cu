@@ -230,7 +230,7 @@ WorkSplit plan_work_split(long long tiles, int k_tiles, int max_workers, double 
     return WorkSplit{cost_split, max_workers, false};
 }
 
-template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, bool EPI_EX = false, int EPI_WARPS = 0>
+template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int EPI_EX = kEpiPlain, int EPI_WARPS = 0>
 int launch_gemm(DeviceCtx* c, int variant, GemmParams& params, const nvfp4_gemm_config& cf, cudaStream_t stream, const char* name) {
     const int grid_request = cf.grid;
     using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, 1, EPI_WARPS>;
@@ -298,7 +298,7 @@ int launch_gemm(DeviceCtx* c, int variant, GemmParams& params, const nvfp4_gemm_
 }
 
 // Cluster split-K launch: one cluster of KS CTAs per 128 x BN output tile.
-template <int BN, int STAGES, int EPI_KB, int KS, bool EPI_EX = false>
+template <int BN, int STAGES, int EPI_KB, int KS, int EPI_EX = kEpiPlain>
 int launch_gemm_splitk(DeviceCtx* c, int variant, GemmParams& params, cudaStream_t stream, const char* name) {
     using S = GemmSmem<1, BN, STAGES, false, EPI_KB, KS>;
     auto kernel = gemm_nvfp4_kernel<1, BN, STAGES, false, EPI_KB, KS, EPI_EX>;
@@ -335,10 +335,11 @@ int launch_gemm_splitk(DeviceCtx* c, int variant, GemmParams& params, cudaStream
 
 // Decode launch: one cluster of KS CTAs per 128 output columns.
 template <int BT, int STAGES, int KS>
-int launch_gemm_decode(DeviceCtx* c, int variant, const GemmParams& params, bool epi, cudaStream_t stream, const char* name) {
+int launch_gemm_decode(DeviceCtx* c, int variant, const GemmParams& params, int epi, cudaStream_t stream, const char* name) {
     using S = DecodeSmem<BT, STAGES, KS>;
-    auto kernel = epi ? gemm_decode_kernel<BT, STAGES, KS, true> : gemm_decode_kernel<BT, STAGES, KS, false>;
-    std::atomic<bool>& attr_set = c->smem_attr_set[24 + 2 * variant + epi];   // (with the rest of what is known of the device: nvfp4_shutdown forgets it)
+    auto kernel = epi == kEpiResidual ? gemm_decode_kernel<BT, STAGES, KS, kEpiResidual>
+                  : epi ? gemm_decode_kernel<BT, STAGES, KS, kEpiExtended> : gemm_decode_kernel<BT, STAGES, KS, kEpiPlain>;
+    std::atomic<bool>& attr_set = c->smem_attr_set[32 + 3 * variant + epi];   // (with the rest of what is known of the device: nvfp4_shutdown forgets it)
     if (!attr_set) {
         CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kDynamicBytes));
         attr_set = true;
@@ -497,7 +498,7 @@ DecodeChoice choose_decode(int m, int n, int k, int l, int num_sms, const nvfp4_
     return DecodeChoice{tokens, split, split == 1 && tiles > num_sms};
 }
 
-int launch_gemm_decode(DeviceCtx* c, const GemmParams& g, const DecodeChoice& d, bool epi, cudaStream_t stream) {
+int launch_gemm_decode(DeviceCtx* c, const GemmParams& g, const DecodeChoice& d, int epi, cudaStream_t stream) {
     if (d.tokens == 32) {
         if (d.split == 8) return launch_gemm_decode<32, 8, 8>(c, 0, g, epi, stream, "gemm_splitk8_decode_t32");
         if (d.split == 4) return launch_gemm_decode<32, 8, 4>(c, 1, g, epi, stream, "gemm_splitk4_decode_t32");
@@ -517,8 +518,14 @@ int launch_gemm_decode(DeviceCtx* c, const GemmParams& g, const DecodeChoice& d,
     return launch_gemm_decode<128, 5, 2>(c, 12, g, epi, stream, "gemm_splitk2_decode_t128");
 }
 
+// What nvfp4_gemm_residual() adds.
+struct Residual {
+    const void* ptr;
+    int64_t row_stride, batch_stride;
+};
+
 int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_epilogue* epi, void* const* c_peers, int n_peers,
-              void* stream_v) {
+              void* stream_v, const Residual* residual = nullptr) {
     const bool to_nvfp4 = epi && epi->output == NVFP4_OUT_NVFP4;
     if (int rc = validate_gemm(p, !to_nvfp4)) return rc;
     if (epi) {
@@ -546,6 +553,12 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
                              (epi->out_sf_perm && epi->out_sf_perm_batch_stride < perm_bytes)))
                 return fail(NVFP4_ERR_INVALID_ARGUMENT, "output batch strides too small or misaligned");
         }
+    }
+
+    if (residual) {
+        if (!residual->ptr || !aligned(residual->ptr, 16)) return fail(NVFP4_ERR_INVALID_ARGUMENT, "residual must be a 16-byte aligned pointer");
+        if (residual->row_stride % 8 || residual->row_stride < 0 || (p->l > 1 && (residual->batch_stride % 8 || residual->batch_stride < 0)))
+            return fail(NVFP4_ERR_INVALID_ARGUMENT, "the residual's strides must be multiples of 8 elements and not negative");
     }
 
     nvfp4_gemm_config cf = {0, 0, 0, 0, 0, 0};
@@ -602,6 +615,11 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
             g.out_sf_perm_block_stride = epi->out_sf_perm_block_stride ? epi->out_sf_perm_block_stride : static_cast<long long>(p->n / 64) * 512;
         }
     }
+    if (residual) {
+        g.residual = static_cast<const __half*>(residual->ptr);
+        g.residual_row_stride = residual->row_stride;
+        g.residual_batch_stride = p->l > 1 ? residual->batch_stride : 0;
+    }
     int set = 0;
     if (int rc = scratch_set_for(c, stream, &set)) return rc;
     g.scratch = c->scratch + static_cast<size_t>(set) * (kScratchBytes / sizeof(float));
@@ -648,7 +666,7 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
                              &g.tma_a)) return rc;
         if (int rc = encode_map(make_key(p->b, kbytes, p->n, p->l, p->b_row_stride, b_bs, kBKBytes, kBM, CU_TENSOR_MAP_DATA_TYPE_UINT8), &g.tma_b)) return rc;
         if (int rc = encode_map(make_sf_key(p->sfb_perm, p->n, p->k, p->l, p->sfb_perm_batch_stride, 1), &g.tma_sfb)) return rc;
-        return launch_gemm_decode(c, g, decode, epi != nullptr, stream);
+        return launch_gemm_decode(c, g, decode, residual ? kEpiResidual : epi ? kEpiExtended : kEpiPlain, stream);
     }
 
     if (epi && to_nvfp4 && g.out_sf_perm && p->m % 128) {
@@ -678,7 +696,8 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
                              &g.tma_b)) return rc;
         if (int rc = encode_map(make_sf_key(p->sfb_perm, p->n, p->k, p->l, p->sfb_perm_batch_stride, bn / 128), &g.tma_sfb)) return rc;
         if (epi) {
-            if (bn == 128 && ks == 2) return launch_gemm_splitk<128, 6, 0, 2, true>(c, 16, g, stream, "gemm_splitk2_n128_s6_epilogue");
+            if (residual && bn == 128 && ks == 2) return launch_gemm_splitk<128, 6, 0, 2, kEpiResidual>(c, 22, g, stream, "gemm_splitk2_n128_s6_residual");
+            if (bn == 128 && ks == 2) return launch_gemm_splitk<128, 6, 0, 2, kEpiExtended>(c, 16, g, stream, "gemm_splitk2_n128_s6_epilogue");
             return fail(NVFP4_ERR_UNSUPPORTED, "the extended epilogue is built for split_k 1 and 2");
         }
         if (bn == 128 && ks == 2) return launch_gemm_splitk<128, 6, 0, 2>(c, 8, g, stream, "gemm_splitk2_n128_s6");
@@ -687,11 +706,17 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
         return launch_gemm_splitk<256, 4, 0, 8>(c, 11, g, stream, "gemm_splitk8_n256_s4");
     }
 
+    if (residual) {
+        if (cg == 2 && bn == 256) return launch_gemm<2, 256, 5, false, 32, kEpiResidual>(c, 23, g, cf, stream, "gemm_2cta_n256_s5_residual");
+        if (cg == 2) return launch_gemm<2, 128, 6, false, 32, kEpiResidual>(c, 24, g, cf, stream, "gemm_2cta_n128_s6_residual");
+        if (bn == 256) return launch_gemm<1, 256, 3, false, 48, kEpiResidual>(c, 25, g, cf, stream, "gemm_1cta_n256_s3_residual");
+        return launch_gemm<1, 128, 4, false, 64, kEpiResidual>(c, 26, g, cf, stream, "gemm_1cta_n128_s4_residual");
+    }
     if (epi) {
-        if (cg == 2 && bn == 256) return launch_gemm<2, 256, 5, false, 32, true>(c, 17, g, cf, stream, "gemm_2cta_n256_s5_epilogue");
-        if (cg == 2) return launch_gemm<2, 128, 6, false, 32, true>(c, 18, g, cf, stream, "gemm_2cta_n128_s6_epilogue");
-        if (bn == 256) return launch_gemm<1, 256, 3, false, 48, true>(c, 19, g, cf, stream, "gemm_1cta_n256_s3_epilogue");
-        return launch_gemm<1, 128, 4, false, 64, true>(c, 20, g, cf, stream, "gemm_1cta_n128_s4_epilogue");
+        if (cg == 2 && bn == 256) return launch_gemm<2, 256, 5, false, 32, kEpiExtended>(c, 17, g, cf, stream, "gemm_2cta_n256_s5_epilogue");
+        if (cg == 2) return launch_gemm<2, 128, 6, false, 32, kEpiExtended>(c, 18, g, cf, stream, "gemm_2cta_n128_s6_epilogue");
+        if (bn == 256) return launch_gemm<1, 256, 3, false, 48, kEpiExtended>(c, 19, g, cf, stream, "gemm_1cta_n256_s3_epilogue");
+        return launch_gemm<1, 128, 4, false, 64, kEpiExtended>(c, 20, g, cf, stream, "gemm_1cta_n128_s4_epilogue");
     }
     if (cg == 2) {
         if (bn == 256 && epilogue == 3) return launch_gemm<2, 256, 4, true, 64>(c, 12, g, cf, stream, "gemm_2cta_n256_s4_tmastore4");
@@ -702,7 +727,7 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
     }
     // (eight epilogue warps for many tiles of one k-tile: see GemmSmem)
     if (bn == 128 && epilogue >= 2 && g.k_tiles == 1 && g.total_units > 2 * c->num_sms)
-        return launch_gemm<1, 128, 5, true, 32, false, 8>(c, 21, g, cf, stream, "gemm_1cta_n128_s5_tmastore");
+        return launch_gemm<1, 128, 5, true, 32, kEpiPlain, 8>(c, 21, g, cf, stream, "gemm_1cta_n128_s5_tmastore");
     if (bn == 128 && epilogue >= 2) return launch_gemm<1, 128, 5, true, 32>(c, 0, g, cf, stream, "gemm_1cta_n128_s5_tmastore");
     if (bn == 128) return launch_gemm<1, 128, 4, false, 64>(c, 1, g, cf, stream, "gemm_1cta_n128_s4_direct");
     if (epilogue >= 2) return launch_gemm<1, 256, 3, true, 32>(c, 2, g, cf, stream, "gemm_1cta_n256_s3_tmastore");
@@ -723,6 +748,14 @@ int nvfp4_gemm(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, void* strea
 int nvfp4_gemm_epilogue(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_epilogue* epi, void* stream_v) {
     if (!epi) return fail(NVFP4_ERR_INVALID_ARGUMENT, "epilogue is NULL (use nvfp4_gemm for the plain fp16 output)");
     return gemm_impl(p, cfg, epi, nullptr, 0, stream_v);
+}
+
+int nvfp4_gemm_residual(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_epilogue* epi, const void* residual,
+                        int64_t residual_row_stride, int64_t residual_batch_stride, void* stream_v) {
+    nvfp4_epilogue none;
+    std::memset(&none, 0, sizeof(none));
+    const Residual r = {residual, residual_row_stride, residual_batch_stride};
+    return gemm_impl(p, cfg, epi ? epi : &none, nullptr, 0, stream_v, &r);
 }
 
 int nvfp4_gemm_allgather(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, void* const* c_peers, int n_peers, void* stream_v) {

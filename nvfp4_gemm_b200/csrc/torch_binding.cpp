@@ -189,11 +189,11 @@ int int_arg(PyObject* o) {
     return static_cast<int>(v);
 }
 
-// gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k) -> status of
-// nvfp4_gemm_epilogue.  out: None for fp16 into data[6], else (packed, sf, sf_permuted) with dense rows.
+// gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k[, residual]) -> status of
+// nvfp4_gemm_epilogue, or of nvfp4_gemm_residual.  out: None for fp16 into data[6], else (packed, sf, sf_permuted) with dense rows.
 PyObject* py_gemm_epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return guarded([&] {
-        if (nargs != 8) raise(PyExc_TypeError, "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k)");
+        if (nargs != 8 && nargs != 9) raise(PyExc_TypeError, "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k[, residual])");
         const Operands o(args[0]);
         o.require_cuda();
         if (args[3] == Py_None && !o.t[6]) raise(PyExc_ValueError, "an fp16 output needs data[6]");
@@ -231,6 +231,14 @@ PyObject* py_gemm_epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             e.out_sf_perm_batch_stride = ((m + 127) / 128) * (n / 64) * 512;
         }
         nvfp4_gemm_config cfg = {int_arg(args[4]), 0, int_arg(args[5]), int_arg(args[6]), int_arg(args[7]), 0};
+        if (const at::Tensor* r = nargs == 9 ? tensor_or_none(args[8]) : nullptr) {
+            if (!r->is_cuda() || r->device() != o.t[0]->device()) raise(PyExc_ValueError, "residual must be on the device of a");
+            if (r->scalar_type() != at::kHalf || r->dim() != 3 || r->size(0) != p.m || r->size(1) != p.n || r->size(2) != p.l || r->stride(1) != 1)
+                raise(PyExc_ValueError, "residual must be fp16 (m, n, l), row-major");
+            const void* const add = r->data_ptr();
+            const int64_t row = p.m > 1 ? r->stride(0) : p.n, batch = batch_stride(*r, 2);
+            return PyLong_FromLong(on_current_stream(*o.t[0], [&](void* stream) { return nvfp4_gemm_residual(&p, &cfg, &e, add, row, batch, stream); }));
+        }
         return PyLong_FromLong(on_current_stream(*o.t[0], [&](void* stream) { return nvfp4_gemm_epilogue(&p, &cfg, &e, stream); }));
     });
 }
@@ -548,7 +556,7 @@ PyMethodDef methods[] = {
     {"matmul", py_matmul, METH_O, "matmul(data) -> status"},
     {"fill_problem", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_fill_problem)), METH_FASTCALL, "fill_problem(data, address)"},
     {"gemm_epilogue", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_gemm_epilogue)), METH_FASTCALL,
-     "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k) -> status"},
+     "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k[, residual]) -> status"},
     {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_route)), METH_FASTCALL,
      "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan) or status"},
     {"plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_plan)), METH_FASTCALL, "plan(experts, number of experts) -> (rows, offsets, plan) or status"},

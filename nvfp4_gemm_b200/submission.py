@@ -59,8 +59,9 @@ _ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_S
 
 
 def gemm_epilogue(data: input_t, bias=None, activation: str = "none", nvfp4_out: bool = False, tile_n: int = 0, grid: int = 0,
-                  cta_group: int = 0, split_k: int = 0, out=None):
-    """The GEMM with the step that follows it fused into its epilogue: ``act(a @ b.T + bias)``.
+                  cta_group: int = 0, split_k: int = 0, out=None, residual=None):
+    """The GEMM with the step that follows it fused into its epilogue: ``act(a @ b.T + bias)``, plus ``residual`` if given
+    (fp16 [M, N, L], added in fp32 ahead of the one rounding; ``data[6]`` itself may be the residual).
 
     ``nvfp4_out=False`` writes fp16 into ``data[6]`` and returns it.  ``nvfp4_out=True`` returns
     the result re-quantised to NVFP4 as ``(packed, sf, sf_permuted)`` -- [M, N/2, L] packed e2m1,
@@ -73,7 +74,7 @@ def gemm_epilogue(data: input_t, bias=None, activation: str = "none", nvfp4_out:
         out = None
     elif out is None:
         out = _empty_nvfp4(data[0].shape[0], data[1].shape[0], data[0].shape[2], data[0].device)
-    _lib.check(_lib.native().gemm_epilogue(data, bias, _ACTIVATIONS[activation], out, tile_n, grid, cta_group, split_k))
+    _lib.check(_lib.native().gemm_epilogue(data, bias, _ACTIVATIONS[activation], out, tile_n, grid, cta_group, split_k, residual))
     return out if nvfp4_out else data[6]
 
 
