@@ -78,6 +78,31 @@ struct ExpertSmem {
     static_assert(BT % (32 * CG) == 0 && kXRows <= 128 && (BT <= 128 || BT == 256), "token tile");
 };
 
+// A worker's tiles: every workers-th of (token tile, block of weight rows).  The table entry of the next one is asked for
+// while the present one is worked on: read when it is needed it kept the MMA issuer waiting 500 cycles a tile.
+struct ExpertTiles {
+    const int4* tiles;
+    int tiles_n, idx, total, step;
+    int4 ahead;
+    __device__ ExpertTiles(const ExpertGemmParams& p, int worker, int workers)
+        : tiles(p.tiles), tiles_n(p.tiles_n), idx(worker - workers), total(*p.tile_count * p.tiles_n), step(workers) {
+        look_ahead(worker);
+    }
+    __device__ __forceinline__ void look_ahead(int i) {
+        if (i < total) ahead = tiles[i / tiles_n];
+    }
+    // the next tile: its entry, which token tile and which block it is
+    __device__ __forceinline__ bool next(int4* t, int* tt, int* nt) {
+        idx += step;
+        if (idx >= total) return false;
+        *t = ahead;
+        *tt = idx / tiles_n;
+        *nt = idx - *tt * tiles_n;
+        look_ahead(idx + step);
+        return true;
+    }
+};
+
 template <int CG, int BT, int STAGES, int EPI_WARPS, int CTAS_PER_SM>
 __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThreads, CTAS_PER_SM) expert_gemm_kernel(const __grid_constant__ ExpertGemmParams p) {
     using S = ExpertSmem<CG, BT, STAGES, EPI_WARPS>;
@@ -132,7 +157,6 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
     }
     const int KT = p.k_tiles;
     const int worker = static_cast<int>(blockIdx.x) / CG, workers = static_cast<int>(gridDim.x) / CG;
-    const int total = *p.tile_count * p.tiles_n;
     const uint64_t timeout = p.timeout_cycles;
     // rows of a tile -> columns of its MMAs
     auto mma_n = [](int rows) { return CG == 2 ? (rows + 31) & ~31 : (rows + 15) & ~15; };
@@ -144,9 +168,10 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
             const uint64_t pol_x = ptx::policy_evict_last();
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int idx = worker; ok && idx < total; idx += workers) {
-                const int tt = idx / p.tiles_n, nt = idx - tt * p.tiles_n;
-                const int4 t = p.tiles[tt];
+            ExpertTiles work(p, worker, workers);
+            int4 t;
+            int tt, nt;
+            while (ok && work.next(&t, &tt, &nt)) {
                 const int n = mma_n(t.z), xrows = n / CG;
                 const int box = xrows <= 16 ? 0 : xrows <= 32 ? 1 : xrows <= 64 ? 2 : 3;
                 const CUtensorMap* map_x = &p.tma_x[box];
@@ -190,8 +215,11 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
             if (ptx::elect_one()) {
                 uint32_t stage = 0, phase = 0, acc_it = 0, sf_buf = 0;
                 bool ok = true;
-                for (int idx = worker; ok && idx < total; idx += workers) {
-                    const int n = mma_n(p.tiles[idx / p.tiles_n].z);
+                ExpertTiles work(p, worker, workers);
+                int4 t;
+                int tt, nt;
+                while (ok && work.next(&t, &tt, &nt)) {
+                    const int n = mma_n(t.z);
                     const uint32_t idesc = ptx::idesc_nvf4(kBM * CG, 0) | (static_cast<uint32_t>(n >> 3) << 17);
                     const bool two_blocks = n > 128;
                     const uint32_t acc = acc_it & 1u;
@@ -243,9 +271,10 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
         uint8_t* const staging_gen = smem_gen + S::kEpiOff + (warp - 2) * S::kStagingPerWarp;
         const bool gated = p.activation == kExpertSwiglu;
         uint32_t acc_it = 0;
-        for (int idx = worker; idx < total; idx += workers) {
-            const int tt = idx / p.tiles_n, nt = idx - tt * p.tiles_n;
-            const int4 t = p.tiles[tt];
+        ExpertTiles work(p, worker, workers);
+        int4 t;
+        int tt, nt;
+        while (work.next(&t, &tt, &nt)) {
             const int wb = nt * CG + cta_rank;
             const bool exists = CG == 1 || wb * kBM < p.n;     // (n is a multiple of 128: a pair's second half may lie beyond it)
             const float alpha = (p.alpha ? p.alpha[t.x] : 1.f);
@@ -276,15 +305,31 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
             const int chunks = (t.z + 31) >> 5;
             const int shared = !S::kOverlap ? chunks : acc == 0 ? max(chunks - 4, 0) : min(chunks, 4);
             const int first = (S::kOverlap && acc == 0 && chunks > 4) ? 4 : 0;
+            auto chunk_at = [&](int pos) { return pos < shared ? first + pos : (S::kOverlap && acc == 0) ? pos - shared : pos; };
+            // Two chunks of a group go to registers together: with two groups these are all that the accumulators share, and
+            // the hand-back does not wait for anything to be converted or stored.
             bool released = false;
-            for (int pos = group; pos < chunks; pos += kGroups) {
-                if (!released && pos >= shared) { release_acc(); released = true; }
-                const int chunk = pos < shared ? first + pos : (S::kOverlap && acc == 0) ? pos - shared : pos;
-                uint32_t v[32];
-                ptx::tc_ld_16lanes_32cols(t_acc + chunk * 32, v);
-                ptx::tc_ld_16lanes_32cols(t_acc + (16u << 16) + chunk * 32, v + 16);
-                ptx::tc_wait_ld();
-                if (!released && pos + kGroups >= shared) { release_acc(); released = true; }
+            uint32_t held[2][32];
+            for (int i = 0, pos = group; pos < chunks; ++i, pos += kGroups) {
+                uint32_t (&v)[32] = held[0];
+                if ((i & 1) == 0) {
+                    const int pos2 = pos + kGroups;
+                    if (!released && pos >= shared) { release_acc(); released = true; }
+                    const uint32_t at = t_acc + chunk_at(pos) * 32;
+                    ptx::tc_ld_16lanes_32cols(at, held[0]);
+                    ptx::tc_ld_16lanes_32cols(at + (16u << 16), held[0] + 16);
+                    if (pos2 < chunks) {
+                        const uint32_t at2 = t_acc + chunk_at(pos2) * 32;
+                        ptx::tc_ld_16lanes_32cols(at2, held[1]);
+                        ptx::tc_ld_16lanes_32cols(at2 + (16u << 16), held[1] + 16);
+                    }
+                    ptx::tc_wait_ld();
+                    if (!released && pos2 + kGroups >= shared) { release_acc(); released = true; }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = held[1][j];
+                }
+                const int chunk = chunk_at(pos);
                 if (!exists) continue;
                 float z[32];     // [half][8 rows of tokens][column t: even, odd token | column t + 8: even, odd token]
 #pragma unroll
