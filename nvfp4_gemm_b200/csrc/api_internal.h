@@ -56,7 +56,7 @@ struct DeviceCtx {
     std::atomic<bool> scratch_ready{false};   // scratch and counters are allocated and cleared
     int max_pairs = -1;  // CTA pairs that can be co-resident (cluster occupancy), queried once
     int expert_pairs = -1;   // the same for the experts' kernel
-    std::atomic<bool> smem_attr_set[80] = {};   // by kernel variant: 0..26 the tiled kernels, 32.. the decode kernels, 72.. the experts' kernels
+    std::atomic<bool> smem_attr_set[96] = {};   // by kernel variant: 0..26 the tiled kernels, 32.. the decode kernels, 72.. the experts' kernels
 };
 
 // The context of the current device.

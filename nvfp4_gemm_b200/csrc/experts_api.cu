@@ -11,12 +11,12 @@ using namespace nvfp4::host;
 
 // Rows of an expert that the grouped product takes at a time: the form with two CTAs per SM (32) where experts have
 // few rows, CTA pairs (256) where they have more.
-constexpr int kTileFew = 32, kTileMany = 256;
+constexpr int kTileFew = 32, kTileMany = 256;   // (powers of two: PlanParams::tile_shift)
 constexpr int kManyFrom = 16;   // rows per expert, on average
 
 struct PlanSizes {
     int tile_tokens, tile_sf_rows, chunk_tokens, chunks;
-    long long max_tiles, words, sf_rows;
+    long long max_tiles, count_words, words, sf_rows;
 };
 
 int plan_sizes(int tokens, int top_k, int experts, PlanSizes* s) {
@@ -31,13 +31,16 @@ int plan_sizes(int tokens, int top_k, int experts, PlanSizes* s) {
     s->max_tiles = pairs / s->tile_tokens + (pairs < experts ? pairs : experts);
     s->sf_rows = s->max_tiles * s->tile_sf_rows;
     if (pairs > 0x7fffffffll || s->sf_rows > 0x7fffffffll) return fail(NVFP4_ERR_INVALID_ARGUMENT, "problem too large: %lld pairs", pairs);
-    // Chunks of the tokens, one CTA each: one for up to 32 tokens (choice and order in one launch), else at most 148.
-    constexpr int kUnit = 32, kMostChunks = 148;
-    const int units = (tokens + kUnit - 1) / kUnit;
-    s->chunk_tokens = kUnit * ((units + kMostChunks - 1) / kMostChunks);
-    if (s->chunk_tokens < kUnit) s->chunk_tokens = kUnit;
-    s->chunks = (tokens + s->chunk_tokens - 1) / s->chunk_tokens;
-    s->words = 4 + 4 * s->max_tiles + pairs + static_cast<long long>(s->chunks) * experts;
+    // Chunks of the tokens.  Up to 128 tokens are one: choice and order take one launch.  Else one CTA each, 148 at most
+    // (more only where a chunk's pairs would not be counted in 16 bits).
+    constexpr int kUnit = 8, kMostChunks = 148, kOneChunk = 128;
+    int chunk_tokens = tokens <= kOneChunk ? kOneChunk : kUnit * ((tokens + kUnit * kMostChunks - 1) / (kUnit * kMostChunks));
+    if (chunk_tokens < 32) chunk_tokens = 32;
+    if (chunk_tokens > kMaxChunkPairs / top_k) chunk_tokens = kMaxChunkPairs / top_k;
+    s->chunk_tokens = chunk_tokens;
+    s->chunks = (tokens + chunk_tokens - 1) / chunk_tokens;
+    s->count_words = static_cast<long long>(s->chunks) * counts_row(experts) / 2;
+    s->words = 4 + 4 * s->max_tiles + s->count_words + pairs;
     return NVFP4_OK;
 }
 
@@ -52,13 +55,18 @@ PlanParams plan_params(const nvfp4_routing* r, const PlanSizes& s) {
     PlanParams q;
     q.tokens = r->tokens; q.top_k = r->top_k; q.experts = r->experts;
     q.tile_tokens = s.tile_tokens; q.tile_sf_rows = s.tile_sf_rows;
+    q.tile_shift = s.tile_tokens == kTileFew ? 5 : 8;
     q.chunk_tokens = s.chunk_tokens; q.chunks = s.chunks;
+    // all pairs of a chunk at once where 28 KB of bits allow it
+    const int in_chunk = r->tokens < s.chunk_tokens ? r->tokens : s.chunk_tokens;
+    const long long needed = (static_cast<long long>(in_chunk) * r->top_k + 31) / 32, most = 7168 / r->experts;
+    q.bit_words = static_cast<int>(needed < most ? needed : most);
     q.expert = r->expert; q.row = r->row; q.offset = r->offset;
     int* words = static_cast<int*>(r->plan);
     q.tile_count = words;
     q.tiles = reinterpret_cast<int4*>(words + 4);
-    q.sf_row = words + 4 + 4 * s.max_tiles;
-    q.counts = q.sf_row + static_cast<long long>(r->tokens) * r->top_k;
+    q.counts = reinterpret_cast<uint16_t*>(words + 4 + 4 * s.max_tiles);
+    q.sf_row = words + 4 + 4 * s.max_tiles + s.count_words;
     return q;
 }
 
@@ -99,27 +107,53 @@ int empty_plan(const PlanParams& q, cudaStream_t stream) {
     return NVFP4_OK;
 }
 
-constexpr int kRouteThreads = 512;
-
-int place(const PlanParams& q, cudaStream_t stream, const char* name) {
-    if (q.chunks <= 1) return NVFP4_OK;
-    return launch(place_kernel, q.chunks, kRouteThreads, plan_smem_words(q.experts) * sizeof(int), 1, stream, name, q);
+size_t plan_smem(const PlanParams& q) {
+    const int per_expert = (q.bit_words | 1) < 2 ? 2 : (q.bit_words | 1);     // (the place kernel keeps two sums there)
+    return (plan_head_words(q.experts) + static_cast<size_t>(q.experts) * per_expert) * sizeof(int);
 }
 
-template <typename Key>
-int launch_route(const RouteParams& p, const PlanParams& q, cudaStream_t stream, const char* name) {
-    // a warp per token; with groups each warp keeps its token's keys in shared memory (at most 32 KB)
-    const int warps = q.experts <= 256 ? 16 : q.experts <= 512 ? 8 : 4;
-    const size_t plan_bytes = plan_smem_words(q.experts) * sizeof(int);
-    const size_t key_bytes = p.groups > 1 ? static_cast<size_t>(warps) * q.experts * sizeof(Key) : 0;
-    const size_t smem = plan_bytes > key_bytes ? plan_bytes : key_bytes;
-    auto go = [&](auto kernel) { return launch(kernel, q.chunks, 32 * warps, smem, 1, stream, name, p, q); };
-    if (q.experts <= 32) return go(route_kernel<Key, 1>);
-    if (q.experts <= 64) return go(route_kernel<Key, 2>);
-    if (q.experts <= 128) return go(route_kernel<Key, 4>);
-    if (q.experts <= 256) return go(route_kernel<Key, 8>);
-    if (q.experts <= 512) return go(route_kernel<Key, 16>);
-    return go(route_kernel<Key, 32>);
+// Raises a kernel's limit of dynamic shared memory once per device.
+int allow_smem(DeviceCtx* c, int variant, const void* kernel, size_t bytes) {
+    if (bytes > 48 * 1024 && !c->smem_attr_set[variant]) {
+        CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        c->smem_attr_set[variant] = true;
+    }
+    return NVFP4_OK;
+}
+
+int place(DeviceCtx* c, const PlanParams& q, cudaStream_t stream, const char* name) {
+    if (q.chunks <= 1) return NVFP4_OK;
+    if (int rc = allow_smem(c, 74, reinterpret_cast<const void*>(place_kernel), plan_smem(q))) return rc;
+    return launch(place_kernel, (q.chunks + kPlaceCluster - 1) / kPlaceCluster * kPlaceCluster, kPlaceThreads, plan_smem(q), kPlaceCluster, stream, name, q);
+}
+
+template <bool BY_LOGIT, int VPL>
+int launch_route(DeviceCtx* c, int variant, RouteParams p, const PlanParams& q, cudaStream_t stream, const char* name) {
+    // A warp per token.  Each has 128 words for candidates; with groups room for all keys, in 64 bits: at most 64 KB.
+    constexpr int kMost = route_threads(VPL) / 32;
+    p.key_words = p.groups > 1 && 2 * q.experts > 128 ? (2 * q.experts + 3) & ~3 : 128;
+    const int in_chunk = q.tokens < q.chunk_tokens ? q.tokens : q.chunk_tokens;
+    // One chunk: up to eight CTAs, so that a scheduler has few tokens to issue for (32 tokens of 256 experts: 7.4 us, in one CTA 11.3).
+    const int most_ctas = q.chunks == 1 ? 8 : 1;
+    p.chunk_ctas = (in_chunk + 3) / 4 < most_ctas ? (in_chunk + 3) / 4 : most_ctas;
+    int warps = (in_chunk + p.chunk_ctas - 1) / p.chunk_ctas;
+    warps = warps < 8 ? 8 : warps > kMost ? kMost : warps;
+    const size_t key_bytes = (plan_head_words(q.experts) + static_cast<size_t>(warps) * p.key_words) * sizeof(int);
+    const size_t smem = plan_smem(q) > key_bytes ? plan_smem(q) : key_bytes;
+    auto kernel = route_kernel<BY_LOGIT, VPL>;
+    if (int rc = allow_smem(c, variant, reinterpret_cast<const void*>(kernel), smem)) return rc;
+    return launch(kernel, q.chunks * p.chunk_ctas, 32 * warps, smem, p.chunk_ctas, stream, name, p, q);
+}
+
+template <bool BY_LOGIT>
+int launch_route(DeviceCtx* c, const RouteParams& p, const PlanParams& q, cudaStream_t stream, const char* name) {
+    constexpr int kFirst = BY_LOGIT ? 76 : 82;
+    if (q.experts <= 32) return launch_route<BY_LOGIT, 1>(c, kFirst, p, q, stream, name);
+    if (q.experts <= 64) return launch_route<BY_LOGIT, 2>(c, kFirst + 1, p, q, stream, name);
+    if (q.experts <= 128) return launch_route<BY_LOGIT, 4>(c, kFirst + 2, p, q, stream, name);
+    if (q.experts <= 256) return launch_route<BY_LOGIT, 8>(c, kFirst + 3, p, q, stream, name);
+    if (q.experts <= 512) return launch_route<BY_LOGIT, 16>(c, kFirst + 4, p, q, stream, name);
+    return launch_route<BY_LOGIT, 32>(c, kFirst + 5, p, q, stream, name);
 }
 
 template <int CG, int BT, int STAGES, int EPI_WARPS, int CTAS_PER_SM>
@@ -205,10 +239,14 @@ int nvfp4_route(const nvfp4_router* o, const nvfp4_routing* r, void* stream_v) {
     p.renormalize = o->renormalize ? 1 : 0;
     p.scale = o->scale;
     p.weights = o->weights;
+    const int per = r->experts / o->groups;
+    p.per_magic = ((1 << 20) + per - 1) / per;
+    p.group_lanes = 32;
+    while (p.group_lanes * o->groups > 32) p.group_lanes /= 2;
     // the order of the logits is that of the scores where nothing is added to them
     const bool by_logit = !o->bias && (o->groups == 1 || o->group_top == 1);
-    if (int rc = by_logit ? launch_route<uint32_t>(p, q, stream, "route") : launch_route<uint64_t>(p, q, stream, "route_64bit")) return rc;
-    return place(q, stream, "route_place");
+    if (int rc = by_logit ? launch_route<true>(c, p, q, stream, "route_by_logits") : launch_route<false>(c, p, q, stream, "route_by_scores")) return rc;
+    return place(c, q, stream, "route_place");
 }
 
 int nvfp4_plan_experts(const nvfp4_routing* r, void* stream_v) {
@@ -220,8 +258,9 @@ int nvfp4_plan_experts(const nvfp4_routing* r, void* stream_v) {
     if (int rc = check_device(&c)) return rc;
     const PlanParams q = plan_params(r, s);
     if (r->tokens == 0) return empty_plan(q, stream);
-    if (int rc = launch(plan_kernel, q.chunks, kRouteThreads, plan_smem_words(q.experts) * sizeof(int), 1, stream, "plan_experts", q)) return rc;
-    return place(q, stream, "plan_experts_place");
+    if (int rc = allow_smem(c, 75, reinterpret_cast<const void*>(plan_kernel), plan_smem(q))) return rc;
+    if (int rc = launch(plan_kernel, q.chunks, kPlaceThreads, plan_smem(q), 1, stream, "plan_experts", q)) return rc;
+    return place(c, q, stream, "plan_experts_place");
 }
 
 int nvfp4_quantize_routed(const void* x, int32_t x_is_bf16, int64_t x_row_stride, int32_t k, const nvfp4_routing* r, void* packed,

@@ -16,8 +16,6 @@
 namespace nvfp4 {
 
 constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
-constexpr int kPlanPairs = 256;      // pairs ranked at a time: a word of bits per 32 of them and expert
-constexpr int kPlanWords = kPlanPairs / 32;
 
 enum Scoring : int { kScoreSoftmax = 0, kScoreSigmoid = 1 };
 enum LogitType : int { kLogitFp16 = 0, kLogitBf16 = 1, kLogitFp32 = 2 };
@@ -31,19 +29,29 @@ struct RouteParams {
     int renormalize;
     float scale;
     float* weights;                // [tokens][top_k]
+    int chunk_ctas;                // CTAs (a cluster) that share a chunk
+    int key_words;                 // shared memory of a warp, a multiple of 4
+    int per_magic;                 // e * per_magic >> 20 is the group of expert e < 1024
+    int group_lanes;               // lanes that judge a group: 32 / groups, rounded down to a power of two
 };
-// The plan's memory.  `plan` words: tile count, 3 unused, tiles {expert, first row, rows, 0}, scale rows [tokens][top_k],
-// counts [chunks][experts].
+// Counts of a chunk: 16 bits an expert, whole 32-byte sectors.
+__host__ __device__ constexpr int counts_row(int experts) { return (experts + 15) & ~15; }
+constexpr int kMaxChunkPairs = 65535;
+constexpr int kPlaceThreads = 512;
+
+// The plan's memory: the word of the tile count, 3 unused, tiles {expert, first row, rows, 0}, the chunks' counts, scale rows [tokens][top_k].
 struct PlanParams {
-    int tokens, top_k, experts, tile_tokens, tile_sf_rows;
+    int tokens, top_k, experts;
+    int tile_tokens, tile_shift, tile_sf_rows;     // rows of a tile (a power of two, and which), of its scales
     int chunk_tokens, chunks;
+    int bit_words;    // words of bits per expert: pairs are ranked 32 times as many at a time
     int* expert;      // [tokens][top_k]
     int* row;         // [tokens][top_k]
     int* offset;      // [experts + 1]
     int* tile_count;
     int4* tiles;
     int* sf_row;      // [tokens][top_k]
-    int* counts;
+    uint16_t* counts; // [chunks][counts_row(experts)]
 };
 
 // ------------------------------------------------------------------------------------------------ choice
@@ -59,6 +67,7 @@ __device__ __forceinline__ uint64_t key_of(double v) {
 __device__ __forceinline__ double value_of(uint64_t key) {
     return __longlong_as_double(static_cast<long long>(key >> 63 ? key & 0x7fffffffffffffffull : ~key));
 }
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 // Largest key of the warp; lanes that do not hold it get the same value.
 __device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
@@ -79,83 +88,121 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // A logit as the router sees it: NaN and -inf mark an expert that cannot be chosen, +inf counts as the largest number.
+__device__ __forceinline__ float as_logit(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
 __device__ __forceinline__ float load_logit(const RouteParams& p, long long at) {
-    float x;
-    if (p.logit_type == kLogitFp32) x = static_cast<const float*>(p.logits)[at];
-    else if (p.logit_type == kLogitBf16) x = __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]);
-    else x = __half2float(static_cast<const __half*>(p.logits)[at]);
-    return x != x ? -INFINITY : fminf(x, 3.402823466e38f);
+    if (p.logit_type == kLogitFp32) return as_logit(static_cast<const float*>(p.logits)[at]);
+    if (p.logit_type == kLogitBf16) return as_logit(__bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]));
+    return as_logit(__half2float(static_cast<const __half*>(p.logits)[at]));
+}
+// A lane's logits of a token as they stand in memory (all loads on their way together: with a look at the type at each, one load
+// waited for the other), and as numbers.
+template <int VPL>
+__device__ __forceinline__ void load_raw(const RouteParams& p, long long at, int lane, int experts, uint32_t (&raw)[VPL]) {
+    if (p.logit_type == kLogitFp32) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) raw[i] = i * 32 + lane < experts ? static_cast<const uint32_t*>(p.logits)[at + i * 32 + lane] : 0u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) raw[i] = i * 32 + lane < experts ? static_cast<const uint16_t*>(p.logits)[at + i * 32 + lane] : 0u;
+    }
+}
+template <int VPL>
+__device__ __forceinline__ void as_logits(const RouteParams& p, int lane, int experts, const uint32_t (&raw)[VPL], float (&x)[VPL]) {
+    if (p.logit_type == kLogitFp32) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = as_logit(__uint_as_float(raw[i]));
+    } else if (p.logit_type == kLogitBf16) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = as_logit(__uint_as_float(raw[i] << 16));
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) x[i] = as_logit(__half2float(__ushort_as_half(static_cast<unsigned short>(raw[i]))));
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane >= experts) x[i] = -INFINITY;
 }
 
-// The choice of one token by one warp: lane holds experts lane, lane + 32, ...  Slot j's expert and weight end
-// in lane j.  Key: uint32_t where the order of the logits is the order of the choice (no bias, and groups judged by
-// their best), else uint64_t, the choice score in 64 bits: two scores may be nearer to each other than 32 bits
-// show, and the experts that are taken must not depend on it.
+// Takes the key out of the warp's keys that is top_key, the one of the lowest expert where several are: that expert.  (Each key is compared
+// with the place that is to go: picked by an index the keys would live in local memory.)
 template <typename Key, int VPL>
-__device__ __forceinline__ void choose(const RouteParams& p, const PlanParams& q, long long token, int lane, Key* group_keys, int& expert,
-                                       float& weight) {
-    constexpr bool kByLogit = sizeof(Key) == 4;
+__device__ __forceinline__ uint32_t take(Key (&key)[VPL], Key top_key, int lane) {
+    uint32_t mine = 0xffffffffu;
+#pragma unroll
+    for (int i = VPL - 1; i >= 0; --i)
+        if (key[i] == top_key) mine = i * 32 + lane;
+    const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+        if (e == static_cast<uint32_t>(i * 32 + lane)) key[i] = 0;
+    return e;
+}
+
+// The choice of one token by one warp: lane holds experts lane, lane + 32, ...
+//
+// Keys.  Where the order of the logits is the order of the choice (no bias, and groups judged by their best) the keys
+// are those of the logits, and exact.  Otherwise two scores may be nearer to each other than 32 bits show, and which
+// experts are taken must not depend on how an exponential rounds.  The scores are computed in 32 bits all the same, with a
+// bound on their error, and every decision is checked against it: where two neighbours of the ranking are not further
+// apart than the bound allows, the candidates' scores are computed and ranked in 64 bits; where groups are not, the token
+// is chosen again in 64 bits (choose_exactly).
+//
+// Ranking.  The top_k largest keys are not below the top_k-th largest of the lanes' maxima.  What is not below it, seldom much
+// more than top_k keys, is put side by side, one to a lane, and each counts those ahead of it.  (Taking the largest top_k
+// times from all lanes' keys took 919 instructions a token of 256 experts, and waited for most of them.)
+
+// The same in 64 bits and by taking the largest again and again, for the few tokens that need it: apart from the other, so that its
+// registers are not the kernel's.  Slot j's expert and its logit end in lane j.  keys: experts words of 64 bits of shared memory (with
+// groups).
+template <bool BY_LOGIT, int VPL>
+__device__ __noinline__ int choose_exactly(const RouteParams& p, const PlanParams& q, long long token, int lane, uint64_t* keys, int& expert,
+                                            float& logit) {
     float x[VPL];
-    Key key[VPL];
+    uint64_t key[VPL];
     float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const int e = i * 32 + lane;
-        x[i] = e < q.experts ? load_logit(p, token * p.logits_row_stride + e) : -INFINITY;
-        top = fmaxf(top, x[i]);
+    {
+        uint32_t raw[VPL];
+        load_raw<VPL>(p, token * p.logits_row_stride, lane, q.experts, raw);
+        as_logits<VPL>(p, lane, q.experts, raw, x);
     }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) top = fmaxf(top, x[i]);
     double total = 0.0;    // softmax: sum of exp(x - top)
-    if (p.scoring == kScoreSoftmax) {
-        const uint32_t t = warp_max(key_of(top));
-        top = __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
-        if constexpr (kByLogit) {
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) sum += x[i] == -INFINITY ? 0.f : expf(x[i] - top);
-            total = warp_sum(sum);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) total += x[i] == -INFINITY ? 0.0 : exp(static_cast<double>(x[i]) - top);
-            total = warp_sum(total);
-        }
+    if (!BY_LOGIT && p.scoring == kScoreSoftmax) {
+        top = value_of(warp_max(key_of(top)));
+#pragma unroll 1
+        for (int i = 0; i < VPL; ++i) total += x[i] == -INFINITY ? 0.0 : exp(static_cast<double>(x[i]) - top);
+        total = warp_sum(total);
     }
-    auto score = [&](float v) {
-        return p.scoring == kScoreSoftmax ? exp(static_cast<double>(v) - top) / total : 1.0 / (1.0 + exp(-static_cast<double>(v)));
-    };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < VPL; ++i) {
         const int e = i * 32 + lane;
-        if constexpr (kByLogit) {
-            key[i] = x[i] == -INFINITY ? 0u : key_of(x[i]);
-        } else {
-            double c = -INFINITY;
-            if (x[i] != -INFINITY) c = score(x[i]) + (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
-            key[i] = c == c && c != -INFINITY ? key_of(c) : 0ull;     // (a bias of -inf or NaN masks its expert too)
-        }
+        double c = x[i];
+        if (!BY_LOGIT && x[i] != -INFINITY)
+            c = (p.scoring == kScoreSoftmax ? exp(static_cast<double>(x[i]) - top) / total : 1.0 / (1.0 + exp(-static_cast<double>(x[i])))) +
+                (p.bias ? static_cast<double>(p.bias[e]) : 0.0);
+        key[i] = c == c && c != -INFINITY ? key_of(c) : 0ull;     // (a bias of -inf or NaN masks its expert too)
     }
     if (p.groups > 1) {
-        // keys to shared memory; lane g judges group g and the warp takes the best top_groups of them
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-            if (i * 32 + lane < q.experts) group_keys[i * 32 + lane] = key[i];
+            if (i * 32 + lane < q.experts) keys[i * 32 + lane] = key[i];
         __syncwarp();
         const int per = q.experts / p.groups;
-        Key mine = 0;
+        uint64_t mine = 0;
         if (lane < p.groups) {
-            Key first = 0, second = 0;
+            uint64_t first = 0, second = 0;
             for (int i = 0; i < per; ++i) {
-                const Key k = group_keys[lane * per + i];
+                const uint64_t k = keys[lane * per + i];
                 if (k > first) { second = first; first = k; }
                 else if (k > second) second = k;
             }
-            mine = first;
-            if constexpr (!kByLogit)
-                if (p.group_top == 2 && second) mine = key_of(value_of(first) + value_of(second));
+            mine = !BY_LOGIT && p.group_top == 2 && second ? key_of(value_of(first) + value_of(second)) : first;
         }
         uint32_t kept = 0;
         for (int g = 0; g < p.top_groups; ++g) {
-            const Key best = warp_max(mine);
+            const uint64_t best = warp_max(mine);
             if (best == 0) break;
             const int at = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
             kept |= 1u << at;
@@ -166,48 +213,247 @@ __device__ __forceinline__ void choose(const RouteParams& p, const PlanParams& q
             const int e = i * 32 + lane;
             if (e < q.experts && !(kept >> (e / per) & 1u)) key[i] = 0;
         }
+        __syncwarp();
     }
     expert = -1;
-    float logit = 0.f;
-    for (int j = 0; j < q.top_k; ++j) {
-        Key best = key[0];
-        int at = 0;
+    int n = 0;
+    for (; n < q.top_k; ++n) {
+        uint64_t best = key[0];
 #pragma unroll
-        for (int i = 1; i < VPL; ++i)
-            if (key[i] > best) { best = key[i]; at = i; }
-        const Key top_key = warp_max(best);
+        for (int i = 1; i < VPL; ++i) best = key[i] > best ? key[i] : best;
+        const uint64_t top_key = warp_max(best);
         if (top_key == 0) break;
-        // ties: the lowest index, over all lanes
-        const uint32_t e = __reduce_min_sync(0xffffffffu, best == top_key ? static_cast<uint32_t>(at * 32 + lane) : 0xffffffffu);
-        const int owner = e & 31, slot = e >> 5;
-        float l = 0.f;
+        const uint32_t e = take(key, top_key, lane);
+        if (lane == n) expert = static_cast<int>(e);
+    }
+    logit = expert >= 0 ? load_logit(p, token * p.logits_row_stride + expert) : 0.f;
+    return n;
+}
+
+// Rank of this lane's key among `of` keys of shared memory (16-byte aligned, the last four filled up with zeros): larger ones, and
+// as large ones of a lower place.
+__device__ __forceinline__ int rank_of(uint32_t mine, int place, const uint32_t* of, int count) {
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; j += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(of + j);
+        rank += (o.x > mine || (o.x == mine && j < place)) + (o.y > mine || (o.y == mine && j + 1 < place)) +
+                (o.z > mine || (o.z == mine && j + 2 < place)) + (o.w > mine || (o.w == mine && j + 3 < place));
+    }
+    return rank;
+}
+
+// x: the token's logits.  keys: shared memory of this warp (p.key_words, 16-byte aligned).  A lane whose slot is not negative has the
+// expert of that slot; slots that no lane has are nobody's.  Returns how many there are.
+template <bool BY_LOGIT, int VPL>
+__device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q, long long token, int lane, const float (&x)[VPL], const float (&bias)[VPL],
+                                      uint32_t* keys, int& slot, int& expert, float& weight) {
+    uint32_t key[VPL];
+    float top = 0.f, total = 1.f;    // softmax: the largest logit, sum of exp(x - top)
+    [[maybe_unused]] float t[VPL];   // scores
+    if (p.scoring == kScoreSoftmax) {
+        top = x[0];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (i == slot) {
-                l = x[i];
-                if (lane == owner) key[i] = 0;
+        for (int i = 1; i < VPL; ++i) top = fmaxf(top, x[i]);
+        top = value_of(warp_max(key_of(top)));
+    }
+    // (a branch around each loop, not a choice in it: both sides of a choice are computed)
+    if (p.scoring == kScoreSoftmax) {
+        if (!BY_LOGIT || !p.renormalize) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                t[i] = x[i] == -INFINITY ? 0.f : __expf(x[i] - top);
+                sum += t[i];
             }
-        l = __shfl_sync(0xffffffffu, l, owner);
-        if (lane == j) { expert = static_cast<int>(e); logit = l; }
+            total = warp_sum(sum);
+            if constexpr (!BY_LOGIT) {
+                const float inv = __fdividef(1.f, total);
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) t[i] *= inv;
+            }
+        }
+    } else if constexpr (!BY_LOGIT) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const float u = __expf(-fabsf(x[i]));
+            t[i] = __fdividef(x[i] >= 0.f ? 1.f : u, 1.f + u);
+        }
     }
-    double s = expert >= 0 ? score(logit) : 0.0;
+    float apart = 0.f;    // decisions are sure where the values are further apart than this
+    if constexpr (BY_LOGIT) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) key[i] = x[i] == -INFINITY ? 0u : key_of(x[i]);
+    } else {
+        // Errors of a score s, in units of 2^-24 of the largest: four for the exponential, one for its argument (times s, at most
+        // 0.37), five for the quotient, VPL + 5 for the softmax's total; then one of the choice.  Two compared values of two scores
+        // each: four times that.
+        uint32_t most = 0u;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const float c = t[i] + bias[i];
+            const bool available = x[i] != -INFINITY && c == c && c != -INFINITY;          // (a bias of -inf or NaN masks its expert too)
+            key[i] = available ? key_of(c) : 0u;
+            most = max(most, available ? __float_as_uint(fabsf(c)) : 0u);
+        }
+        const float units = p.scoring == kScoreSoftmax ? __fdividef(VPL + 16.f, total) : 10.f;      // (the largest softmax score is 1 / total)
+        apart = 4.f * 5.9604645e-8f * (units + __uint_as_float(__reduce_max_sync(0xffffffffu, most)));
+    }
+    if (p.groups > 1) {
+        // 32 / (groups rounded up to a power of two) lanes judge a group; rows of keys one word apart, against bank conflicts
+        __syncwarp();
+        const int per = q.experts / p.groups;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int e = i * 32 + lane;
+            if (e < q.experts) keys[e + (e * p.per_magic >> 20)] = key[i];
+        }
+        __syncwarp();
+        const int lanes = p.group_lanes, g = lane / lanes;
+        uint32_t first = 0, second = 0;
+        if (g < p.groups)
+            for (int i = lane & (lanes - 1); i < per; i += lanes) {
+                const uint32_t k = keys[g * (per + 1) + i];
+                second = max(second, min(first, k));
+                first = max(first, k);
+            }
+        for (int s = 1; s < lanes; s <<= 1) {
+            const uint32_t f = __shfl_xor_sync(0xffffffffu, first, s), u = __shfl_xor_sync(0xffffffffu, second, s);
+            second = max(min(first, f), max(second, u));
+            first = max(first, f);
+        }
+        uint32_t mine = first;
+        if (!BY_LOGIT && p.group_top == 2 && second) mine = key_of(value_of(first) + value_of(second));
+        // rank of the group among all: better ones, and as good ones of a lower index
+        int rank = 0;
+#pragma unroll 8
+        for (int h = 0; h < p.groups; ++h) {
+            const uint32_t other = __shfl_sync(0xffffffffu, mine, h * lanes);
+            rank += other > mine || (other == mine && h < g);
+        }
+        const bool keep = g < p.groups && rank < p.top_groups;
+        const uint32_t heads = __ballot_sync(0xffffffffu, keep && (lane & (lanes - 1)) == 0);      // bit h * lanes: group h is kept
+        if constexpr (!BY_LOGIT) {
+            const uint32_t worst = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu);
+            const uint32_t best = __reduce_max_sync(0xffffffffu, keep || g >= p.groups ? 0u : mine);
+            if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > apart)) apart = INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int e = i * 32 + lane;
+            if (e < q.experts && !(heads >> ((e * p.per_magic >> 20) * lanes) & 1u)) key[i] = 0;
+        }
+        __syncwarp();
+    }
+    // candidates, one to a lane: cand holds their keys, ids their experts
+    uint32_t* const cand = keys;
+    uint32_t* const ids = keys + 32;
+    const bool unsure_group = !BY_LOGIT && apart == INFINITY;
+    int n = 0, rank = 0;
+    uint32_t mine = 0u;
+    expert = -1;
+    if constexpr (VPL == 1) {
+        mine = key[0];
+        expert = lane;
+        cand[lane] = mine;
+        n = __popc(__ballot_sync(0xffffffffu, mine != 0));
+        __syncwarp();
+        rank = rank_of(mine, lane, cand, 32);
+    } else {
+        const int least = q.top_k + (BY_LOGIT ? 0 : 1);       // (by scores the next one is needed too, to be told apart)
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < VPL; ++i) best = max(best, key[i]);
+        cand[lane] = best;
+        __syncwarp();
+        int ahead = 0;      // lanes whose best is larger: the least-th largest is the smallest that fewer than that are ahead of
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(cand + j);
+            ahead += (o.x > best) + (o.y > best) + (o.z > best) + (o.w > best);
+        }
+        uint32_t floor_key = least > 32 ? 0u : __reduce_min_sync(0xffffffffu, ahead < least ? best : 0xffffffffu);
+        if (!BY_LOGIT && floor_key) floor_key = key_of(value_of(floor_key) - apart);
+        floor_key = max(floor_key, 1u);
+        __syncwarp();
+        cand[lane] = 0u;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const uint32_t b = __ballot_sync(0xffffffffu, key[i] >= floor_key);
+            const int pos = n + __popc(b & ((1u << lane) - 1u));
+            if (key[i] >= floor_key && pos < 32) { cand[pos] = key[i]; ids[pos] = i * 32 + lane; }
+            n += __popc(b);
+        }
+        __syncwarp();
+        if (lane < n) { mine = cand[lane]; expert = ids[lane]; }
+        rank = rank_of(mine, lane, cand, min(n, 32));
+    }
+    float logit = 0.f;
+    if (n > 32 || unsure_group) {
+        // more alike than lanes, or groups that 32 bits cannot tell apart
+        __syncwarp();
+        n = choose_exactly<BY_LOGIT, VPL>(p, q, token, lane, reinterpret_cast<uint64_t*>(keys), expert, logit);
+        slot = expert >= 0 ? lane : -1;
+    } else {
+        if constexpr (!BY_LOGIT) {
+            uint32_t* const sorted = keys + 64;
+            if (mine) sorted[rank] = mine;
+            __syncwarp();
+            bool sure = true;
+            if (lane < q.top_k && lane + 1 < n) sure = value_of(sorted[lane]) - value_of(sorted[lane + 1]) > apart;
+            if (!__all_sync(0xffffffffu, sure)) {
+                double all = 1.0;
+                if (p.scoring == kScoreSoftmax) {
+                    all = 0.0;
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) all += x[i] == -INFINITY ? 0.0 : exp(static_cast<double>(x[i]) - top);
+                    all = warp_sum(all);
+                }
+                uint64_t exact = 0;
+                if (mine) {
+                    const double l = load_logit(p, token * p.logits_row_stride + expert);
+                    exact = key_of((p.scoring == kScoreSoftmax ? exp(l - top) / all : 1.0 / (1.0 + exp(-l))) + (p.bias ? static_cast<double>(p.bias[expert]) : 0.0));
+                }
+                rank = 0;
+                for (int j = 0; j < 32; ++j) {
+                    const uint64_t other = __shfl_sync(0xffffffffu, exact, j);
+                    rank += other > exact || (other == exact && j < lane);
+                }
+            }
+        }
+        slot = mine && rank < q.top_k ? rank : -1;
+        if (slot >= 0) logit = BY_LOGIT ? value_of(mine) : load_logit(p, token * p.logits_row_stride + expert);
+    }
+    float s = 0.f;
+    if (slot >= 0) {
+        const float a = expf(p.scoring == kScoreSoftmax ? logit - top : -fabsf(logit));
+        s = p.scoring == kScoreSoftmax ? a / total : (logit >= 0.f ? 1.f : a) / (1.f + a);
+    }
     if (p.renormalize) {
-        const double sum = warp_sum(s);
-        s = sum > 0.0 ? s / sum : 0.0;
+        const float sum = warp_sum(s);
+        if (sum > 1e-30f) {
+            s /= sum;
+        } else {       // scores that 32 bits hardly hold: their ratios in 64
+            const double far = slot < 0 ? 0.0 : p.scoring == kScoreSoftmax ? exp(static_cast<double>(logit) - top) : 1.0 / (1.0 + exp(-static_cast<double>(logit)));
+            const double all = warp_sum(far);
+            s = all > 0.0 ? static_cast<float>(far / all) : 0.f;
+        }
     }
-    weight = static_cast<float>(s * p.scale);
+    weight = s * p.scale;
+    return min(n, q.top_k);
 }
 
 // -------------------------------------------------------------------------------------------------- plan
 // Exclusive sums over the experts of a CTA: first row and first tile of each.  count[e] in, row0[e] / tile0[e] out
 // (both of experts + 1 entries); all threads of the CTA take part.  scratch: 2 x 32 words.
-__device__ __forceinline__ void scan_experts(const int* count, int* row0, int* tile0, int experts, int tile_tokens, int* scratch) {
+__device__ __forceinline__ void scan_experts(const int* count, int* row0, int* tile0, int experts, int tile_shift, int* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int carry_r = 0, carry_t = 0;
     for (int base = 0; base < experts; base += blockDim.x) {
         const int e = base + threadIdx.x;
         const int c = e < experts ? count[e] : 0;
-        int r = c, t = (c + tile_tokens - 1) / tile_tokens;
+        int r = c, t = (c + (1 << tile_shift) - 1) >> tile_shift;
         const int t_own = t;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -216,12 +462,17 @@ __device__ __forceinline__ void scan_experts(const int* count, int* row0, int* t
         }
         if (lane == 31) { scratch[warp] = r; scratch[32 + warp] = t; }
         __syncthreads();
-        int before_r = carry_r, before_t = carry_t;
-        for (int w = 0; w < warps; ++w) {
-            if (w < warp) { before_r += scratch[w]; before_t += scratch[32 + w]; }
-            carry_r += scratch[w];
-            carry_t += scratch[32 + w];
+        // (every warp adds up the warps' sums itself)
+        int wr = lane < warps ? scratch[lane] : 0, wt = lane < warps ? scratch[32 + lane] : 0;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int a = __shfl_up_sync(0xffffffffu, wr, s), b = __shfl_up_sync(0xffffffffu, wt, s);
+            if (lane >= s) { wr += a; wt += b; }
         }
+        const int up_r = __shfl_sync(0xffffffffu, wr, max(warp - 1, 0)), up_t = __shfl_sync(0xffffffffu, wt, max(warp - 1, 0));
+        const int before_r = carry_r + (warp ? up_r : 0), before_t = carry_t + (warp ? up_t : 0);
+        carry_r += __shfl_sync(0xffffffffu, wr, 31);
+        carry_t += __shfl_sync(0xffffffffu, wt, 31);
         if (e < experts) { row0[e] = before_r + r - c; tile0[e] = before_t + t - t_own; }
         __syncthreads();
     }
@@ -229,41 +480,39 @@ __device__ __forceinline__ void scan_experts(const int* count, int* row0, int* t
     __syncthreads();
 }
 
-// Rows of a chunk's pairs.  next[e]: how many pairs of expert e stand before the chunk (changed here); bits: experts x kPlanWords words.
-// Pairs are ranked kPlanPairs at a time by a bit per pair and expert, so that the order is that of the pairs whichever
+// Rows of a chunk's pairs.  next[e]: how many pairs of expert e stand before the chunk (changed here); bits: experts x (bit_words | 1) words.
+// Pairs are ranked 32 * words at a time by a bit per pair and expert, so that the order is that of the pairs whichever
 // thread comes first, and the same expert twice in a token gets two rows.
 __device__ __forceinline__ void place_pairs(const PlanParams& q, long long first_pair, int pairs, const int* row0, const int* tile0, int* next,
                                             uint32_t* bits) {
-    for (int base = 0; base < pairs; base += kPlanPairs) {
-        for (int i = threadIdx.x; i < q.experts * kPlanWords; i += blockDim.x) bits[i] = 0u;
+    const int words = q.bit_words, batch = 32 * words, stride = words | 1;     // (odd: an expert's words and the next one's in other banks)
+    for (int base = 0; base < pairs; base += batch) {
+        const int here = min(batch, pairs - base), used = (here + 31) >> 5;
+        for (int i = threadIdx.x; i < q.experts * stride; i += blockDim.x) bits[i] = 0u;
         __syncthreads();
-        const int here = min(kPlanPairs, pairs - base);
         for (int i = threadIdx.x; i < here; i += blockDim.x) {
             const int e = q.expert[first_pair + base + i];
-            if (e >= 0 && e < q.experts) atomicOr(&bits[e * kPlanWords + (i >> 5)], 1u << (i & 31));
+            if (e >= 0 && e < q.experts) atomicOr(&bits[e * stride + (i >> 5)], 1u << (i & 31));
         }
         __syncthreads();
         for (int i = threadIdx.x; i < here; i += blockDim.x) {
             const int e = q.expert[first_pair + base + i];
             int row = -1, sf_row = -1;
             if (e >= 0 && e < q.experts) {
-                int rank = next[e];
-#pragma unroll
-                for (int w = 0; w < kPlanWords; ++w) {
-                    const uint32_t b = bits[e * kPlanWords + w];
-                    rank += w < (i >> 5) ? __popc(b) : w == (i >> 5) ? __popc(b & ((1u << (i & 31)) - 1u)) : 0;
-                }
+                int rank = next[e] + __popc(bits[e * stride + (i >> 5)] & ((1u << (i & 31)) - 1u));
+#pragma unroll 4
+                for (int w = 0; w < (i >> 5); ++w) rank += __popc(bits[e * stride + w]);
                 row = row0[e] + rank;
-                sf_row = (tile0[e] + rank / q.tile_tokens) * q.tile_sf_rows + rank % q.tile_tokens;
+                sf_row = (tile0[e] + (rank >> q.tile_shift)) * q.tile_sf_rows + (rank & (q.tile_tokens - 1));
             }
             q.row[first_pair + base + i] = row;
             q.sf_row[first_pair + base + i] = sf_row;
         }
+        if (base + batch >= pairs) break;
         __syncthreads();
         for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
             int n = 0;
-#pragma unroll
-            for (int w = 0; w < kPlanWords; ++w) n += __popc(bits[e * kPlanWords + w]);
+            for (int w = 0; w < used; ++w) n += __popc(bits[e * stride + w]);
             next[e] += n;
         }
         __syncthreads();
@@ -279,96 +528,166 @@ __device__ __forceinline__ void write_tables(const PlanParams& q, const int* row
             q.tiles[t] = make_int4(e, r, min(q.tile_tokens, row0[e + 1] - r), 0);
 }
 
-// Shared memory of the plan: counts / next [experts], row0 and tile0 [experts + 1], scan scratch, bits.
-__host__ __device__ constexpr int plan_smem_words(int experts) { return 3 * (experts + 1) + 64 + experts * kPlanWords; }
+// Shared memory of the plan, in words: next, row0 and tile0 [experts + 1], scan scratch, bits.
+__host__ __device__ constexpr int plan_head_words(int experts) { return (3 * (experts + 1) + 64 + 3) & ~3; }
+struct PlanSmem {
+    int *next, *row0, *tile0, *scratch;
+    uint32_t* bits;
+    __device__ PlanSmem(int* smem, int experts)
+        : next(smem), row0(next + experts + 1), tile0(row0 + experts + 1), scratch(tile0 + experts + 1),
+          bits(reinterpret_cast<uint32_t*>(smem + plan_head_words(experts))) {}
+};
 
-// One chunk's share of the order, where the counts of all chunks are known.  Every CTA adds up the counts of all
-// chunks for itself (at most 160 x experts words from L2) instead of a launch between.
-__global__ void __launch_bounds__(512) place_kernel(const PlanParams q) {
+// One chunk's share of the order, where the counts of all chunks are known (16 bits each).  The eight CTAs of a cluster share the work of
+// adding them up: each sums every eighth chunk, over all chunks and over those ahead of the cluster's, and takes the others' sums from their
+// shared memory.  (Each CTA for itself: 148 CTAs read the same 75 KB of 256 experts' counts in 8000 cycles.)
+constexpr int kPlaceCluster = 8;
+__global__ void __launch_bounds__(kPlaceThreads) place_kernel(const PlanParams q) {
     extern __shared__ __align__(16) int plan_smem[];
-    int* next = plan_smem;
-    int* row0 = next + q.experts + 1;
-    int* tile0 = row0 + q.experts + 1;
-    int* scratch = tile0 + q.experts + 1;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(scratch + 64);
+    const PlanSmem s(plan_smem, q.experts);
+    int* const sums = reinterpret_cast<int*>(s.bits);       // [2][experts]: ahead of the cluster's chunks, of all (this CTA's share)
     ptx::grid_dependency_launch_dependents();
     ptx::grid_dependency_wait();
-    const int chunk = blockIdx.x;
-    // (row0 holds the totals until the scan has read them: count and result of an expert belong to one thread)
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
-        int before = 0, all = 0;
-#pragma unroll 8
-        for (int c = 0; c < q.chunks; ++c) {
-            const int n = q.counts[static_cast<long long>(c) * q.experts + e];
-            before += c < chunk ? n : 0;
-            all += n;
+    const int chunk = blockIdx.x, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(ptx::cluster_ctarank()), cluster_first = chunk - rank;
+    const int count_row = counts_row(q.experts);
+    // a warp takes sixteen experts (a sector of a chunk's row), a lane a chunk
+    for (int e0 = (threadIdx.x >> 5) * 16; e0 < q.experts; e0 += (blockDim.x >> 5) * 16) {
+        int before[16] = {}, all[16] = {};
+        for (int c = rank + kPlaceCluster * lane; c < q.chunks; c += kPlaceCluster * 32) {
+            const uint4* src = reinterpret_cast<const uint4*>(q.counts + static_cast<long long>(c) * count_row + e0);
+            const uint4 v0 = src[0], v1 = src[1];
+            const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int n = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+                all[j] += n;
+                before[j] += c < cluster_first ? n : 0;
+            }
         }
-        next[e] = before;
-        row0[e] = all;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int b = __reduce_add_sync(0xffffffffu, before[j]), t = __reduce_add_sync(0xffffffffu, all[j]);
+            if (lane == j && e0 + j < q.experts) { sums[e0 + j] = b; sums[q.experts + e0 + j] = t; }
+        }
     }
-    __syncthreads();
-    scan_experts(row0, row0, tile0, q.experts, q.tile_tokens, scratch);
-    if (chunk == 0) write_tables(q, row0, tile0);
+    ptx::cluster_arrive();
+    // the chunks of this cluster ahead of this one
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kPlaceCluster - 1; ++i)
+            if (i < rank && cluster_first + i < q.chunks) n += q.counts[static_cast<long long>(cluster_first + i) * count_row + e];
+        s.next[e] = n;
+    }
+    ptx::cluster_wait();
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
+        const uint32_t at = ptx::smem_u32(sums + e);
+        int before = s.next[e], all = 0;
+#pragma unroll
+        for (int r = 0; r < kPlaceCluster; ++r) {
+            const uint32_t from = ptx::mapa_u32(at, r);
+            before += static_cast<int>(ptx::ld_shared_cluster_u32(from));
+            all += static_cast<int>(ptx::ld_shared_cluster_u32(from + q.experts * 4));
+        }
+        s.next[e] = before;
+        s.row0[e] = all;
+    }
+    ptx::cluster_arrive();      // the others' sums have been read
+    ptx::cluster_wait();        // (what stands in their place next are this CTA's bits)
+    if (chunk >= q.chunks) return;
+    scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
+    if (chunk == 0) write_tables(q, s.row0, s.tile0);
     const long long first = static_cast<long long>(chunk) * q.chunk_tokens;
     const int tokens = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - first));
-    place_pairs(q, first * q.top_k, tokens * q.top_k, row0, tile0, next, bits);
+    place_pairs(q, first * q.top_k, tokens * q.top_k, s.row0, s.tile0, s.next, s.bits);
 }
 
-// The rest of a CTA that knows its chunk's experts (in global memory, written by this CTA or given): the counts of
-// the chunk, or everything where the chunk is the only one.
-__device__ __forceinline__ void count_and_place(const PlanParams& q, int chunk, int* smem) {
-    int* next = smem;
-    int* row0 = next + q.experts + 1;
-    int* tile0 = row0 + q.experts + 1;
-    int* scratch = tile0 + q.experts + 1;
-    uint32_t* bits = reinterpret_cast<uint32_t*>(scratch + 64);
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) row0[e] = 0;
-    __syncthreads();
+// The rest of a CTA that has counted its chunk's pairs in s.row0: the counts go to the other CTAs, or, where the chunk is the
+// only one, everything is known.
+__device__ __forceinline__ void finish_chunk(const PlanParams& q, int chunk, const PlanSmem& s) {
+    if (q.chunks > 1) {
+        for (int e = threadIdx.x; e < q.experts; e += blockDim.x) q.counts[static_cast<long long>(chunk) * counts_row(q.experts) + e] = static_cast<uint16_t>(s.row0[e]);
+        return;
+    }
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) s.next[e] = 0;
+    scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
+    write_tables(q, s.row0, s.tile0);
+    place_pairs(q, 0, q.tokens * q.top_k, s.row0, s.tile0, s.next, s.bits);
+}
+
+// Adds a chunk's pairs, given in global memory, to s.row0.
+__device__ __forceinline__ void count_pairs(const PlanParams& q, int chunk, const PlanSmem& s) {
     const long long first = static_cast<long long>(chunk) * q.chunk_tokens;
     const int pairs = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - first)) * q.top_k;
     for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
         const int e = q.expert[first * q.top_k + i];
-        if (e >= 0 && e < q.experts) atomicAdd(&row0[e], 1);
+        if (e >= 0 && e < q.experts) atomicAdd(&s.row0[e], 1);
     }
     __syncthreads();
-    if (q.chunks > 1) {
-        for (int e = threadIdx.x; e < q.experts; e += blockDim.x) q.counts[static_cast<long long>(chunk) * q.experts + e] = row0[e];
-        return;
-    }
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) next[e] = 0;
-    scan_experts(row0, row0, tile0, q.experts, q.tile_tokens, scratch);
-    write_tables(q, row0, tile0);
-    place_pairs(q, 0, pairs, row0, tile0, next, bits);
 }
 
-__global__ void __launch_bounds__(512) plan_kernel(const PlanParams q) {
+__global__ void __launch_bounds__(kPlaceThreads) plan_kernel(const PlanParams q) {
     extern __shared__ __align__(16) int plan_smem[];
+    const PlanSmem s(plan_smem, q.experts);
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) s.row0[e] = 0;
+    __syncthreads();
     ptx::grid_dependency_launch_dependents();
     ptx::grid_dependency_wait();
-    count_and_place(q, blockIdx.x, plan_smem);
+    count_pairs(q, blockIdx.x, s);
+    finish_chunk(q, blockIdx.x, s);
 }
 
-// A warp per token, a chunk of tokens per CTA.  Shared memory: the plan's, or before that a row of keys per warp for the groups.
-template <typename Key, int VPL>
-__global__ void __launch_bounds__(512) route_kernel(const RouteParams p, const PlanParams q) {
+// A warp per token; the CTAs of a cluster share a chunk of tokens, and the first of them counts its pairs (and, where it is the only chunk,
+// brings them into order).  The warps' keys stand where the plan's bits come later.
+constexpr int route_threads(int vpl) { return vpl <= 8 ? 1024 : vpl <= 16 ? 512 : 256; }
+template <bool BY_LOGIT, int VPL>
+__global__ void __launch_bounds__(route_threads(VPL)) route_kernel(const RouteParams p, const PlanParams q) {
     extern __shared__ __align__(16) int plan_smem[];
+    const PlanSmem s(plan_smem, q.experts);
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) s.row0[e] = 0;
+    __syncthreads();
     ptx::grid_dependency_launch_dependents();
     ptx::grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    Key* group_keys = reinterpret_cast<Key*>(plan_smem) + warp * q.experts;
-    const long long first = static_cast<long long>(blockIdx.x) * q.chunk_tokens;
-    const int tokens = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - first));
+    uint32_t* const keys = s.bits + warp * p.key_words;
+    const int ctas = p.chunk_ctas, chunk = blockIdx.x / ctas, rank = blockIdx.x - chunk * ctas;
+    const long long chunk_first = static_cast<long long>(chunk) * q.chunk_tokens;
+    const int in_chunk = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - chunk_first));
+    const int share = (in_chunk + ctas - 1) / ctas;
+    const long long first = chunk_first + rank * share;
+    const int tokens = min(share, in_chunk - rank * share);
+    float bias[VPL];
+    uint32_t ahead[VPL];     // the logits of a token are asked for while the one before is worked on
+    if (warp < tokens) load_raw<VPL>(p, (first + warp) * p.logits_row_stride, lane, q.experts, ahead);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) bias[i] = !BY_LOGIT && p.bias && i * 32 + lane < q.experts ? p.bias[i * 32 + lane] : 0.f;
     for (int t = warp; t < tokens; t += warps) {
-        int expert;
+        float x[VPL];
+        as_logits<VPL>(p, lane, q.experts, ahead, x);
+        if (t + warps < tokens) load_raw<VPL>(p, (first + t + warps) * p.logits_row_stride, lane, q.experts, ahead);
+        int slot, expert;
         float weight;
-        choose<Key, VPL>(p, q, first + t, lane, group_keys, expert, weight);
-        if (lane < q.top_k) {
-            q.expert[(first + t) * q.top_k + lane] = expert;
-            p.weights[(first + t) * q.top_k + lane] = weight;
+        const int n = choose<BY_LOGIT, VPL>(p, q, first + t, lane, x, bias, keys, slot, expert, weight);
+        const long long at = (first + t) * q.top_k;
+        if (slot >= 0) {
+            q.expert[at + slot] = expert;
+            p.weights[at + slot] = weight;
         }
+        if (lane >= n && lane < q.top_k) {
+            q.expert[at + lane] = -1;
+            p.weights[at + lane] = 0.f;
+        }
+        __syncwarp();
     }
     __syncthreads();     // (the experts that the other threads wrote are read back from global memory by this CTA)
-    count_and_place(q, blockIdx.x, plan_smem);
+    if (ctas > 1) {
+        ptx::cluster_arrive();     // releases what the CTAs have written
+        ptx::cluster_wait();
+        if (rank != 0) return;
+    }
+    count_pairs(q, chunk, s);
+    finish_chunk(q, chunk, s);
 }
 
 // ------------------------------------------------------------------------------------------ routed quantiser
