@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) gemm_decode_kernel(const __
 #pragma unroll kUnroll
                     for (int h = 0; h < kCols; h += 16) {
                         [[maybe_unused]] uint4 res[2];
-                        if constexpr (EPI_EX == kEpiResidual) load_residual<16>(p, l, row, gcol + h, res);
+                        if constexpr (kHasResidual<EPI_EX>) load_residual<16>(p, l, row, gcol + h, res);
                         float s[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) s[i] = 0.f;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) gemm_decode_kernel(const __
                             }
                         }
                         if constexpr (EPI_EX) bias_act16(p, gcol + h, s);
-                        if constexpr (EPI_EX == kEpiResidual) add_residual16(res, s);
+                        if constexpr (kHasResidual<EPI_EX>) add_fp16x16(res, s);
                         if (!EPI_EX || !p.out_nvfp4) {
                             __half* dst = p.c + l * p.c_batch_stride + static_cast<long long>(row) * p.c_row_stride + gcol + h;
                             *reinterpret_cast<uint4*>(dst) = pack8_fp16(&s[0]);

@@ -54,7 +54,10 @@ enum Activation : int { kActNone = 0, kActRelu = 1, kActSilu = 2 };
 
 // What a kernel does with a finished accumulator: fp16 as it is; bias, activation and NVFP4 output; and the same
 // with a residual.  (A form of its own: the loads and the larger code are not for those that have none.)
-constexpr int kEpiPlain = 0, kEpiExtended = 1, kEpiResidual = 2;
+// kEpiResidualFp16 writes fp16 only, whole tiles by tensor stores.
+constexpr int kEpiPlain = 0, kEpiExtended = 1, kEpiResidual = 2, kEpiResidualFp16 = 3;
+template <int EPI>
+constexpr bool kHasResidual = EPI >= kEpiResidual;
 
 enum GemmStatus : int {
     kStatusOk = 0,
@@ -66,6 +69,7 @@ struct GemmParams {
     CUtensorMap tma_b;   // {K/2 bytes, N rows, L}, box {128, BN/CG, 1},  128B swizzle
     CUtensorMap tma_c;   // {N, M, L} fp16, box {64, 32, 1}, 128B swizzle (TMA-store epilogue)
     CUtensorMap tma_sfa; // permuted scales of A as {128 words, K/64 atoms, row blocks, L}, box {128, 4, 1, 1}
+    CUtensorMap tma_res; // (EPI_EX == kEpiResidualFp16) the residual {N, M, L} fp16, as tma_c
     CUtensorMap tma_sfb; // permuted scales of B, same view, box {128, 4, BN/128, 1}
     __half* c;
     // Fused all-gather (column-parallel multi-GPU): every finished piece of C is also stored into
@@ -110,7 +114,7 @@ constexpr int kPrefetchStages = 2;                  // stages of a CTA's first s
 constexpr int kGlobalExchangeMinSplit = 4;         // cluster split-K: from this split on the partial sums travel through L2
 constexpr int kScratchSlotFloats = kBM * 256;      // one partial-tile slot of the library's scratch (128 x 256 fp32)
 
-template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int KS = 1, int EPI_WARPS = 0>
+template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int KS = 1, int EPI_WARPS = 0, bool RESIDUAL = false>
 struct GemmSmem {
     static constexpr uint32_t kBRows = BN / CG;
     static constexpr uint32_t kABytes = kBM * kBKBytes;
@@ -135,7 +139,9 @@ struct GemmSmem {
     static constexpr uint32_t kStagingPerWarp = kStagingBufs * 32 * 128;
     static constexpr uint32_t kFixBufs = 2;   // barriers of the cluster split-K exchange ("landed", "ready")
     static constexpr uint32_t kEpiOff = STAGES * kStageBytes;
-    static constexpr uint32_t kBarOff = kEpiOff + kEpiBytes;
+    static constexpr uint32_t kBiasOff = kEpiOff + kEpiBytes;          // (residual) each warp's share of the bias: 128 bytes per staging buffer
+    static constexpr uint32_t kBiasPerWarp = RESIDUAL ? kStagingBufs * 128 : 0;
+    static constexpr uint32_t kBarOff = kBiasOff + kEpiWarps * kBiasPerWarp;
     // Cluster split-K: one sender's share of the columns a CTA finalises, and whether the ring holds
     // both the KS - 1 incoming pieces and the KS - 1 outgoing ones (then the exchange uses bulk copies).
     static constexpr uint32_t kPieceBytes = (BN / KS) * kBM * 4;
@@ -146,8 +152,8 @@ struct GemmSmem {
     static constexpr bool kAccOverlap = (BN == 256 && KS == 1);        // see the TMEM column map above
     static constexpr uint32_t kNumAcc = (BN <= 128 || kAccOverlap) ? 2 : 1;
     static constexpr uint32_t kAccStride = kAccOverlap ? BN / 2 : BN;  // TMEM columns between the two accumulators
-    // full[STAGES] empty[STAGES] acc_full[2] acc_empty[2] exchange[kFixBufs] | tmem slot | abort
-    static constexpr uint32_t kNumBars = 2 * STAGES + 4 + kFixBufs;
+    // full[STAGES] empty[STAGES] acc_full[2] acc_empty[2] exchange[kFixBufs] residual[epilogue warps] | tmem slot | abort
+    static constexpr uint32_t kNumBars = 2 * STAGES + 4 + kFixBufs + (RESIDUAL ? kEpiWarps : 0);
     static constexpr uint32_t kBytes = kBarOff + kNumBars * 8 + 16;
     static constexpr uint32_t kDynamicBytes = kBytes + 1024;  // slack for manual 1024-byte alignment
     static_assert(kStageBytes % 1024 == 0, "stage tiles must keep 1024-byte alignment");
@@ -263,40 +269,8 @@ __device__ __forceinline__ uint4 pack8_fp16(const uint32_t* v) {
     return pack8_fp16(f);
 }
 
-// bias and activation on 16 columns from output column gcol on (extended epilogue)
-__device__ __forceinline__ void bias_act16(const GemmParams& p, int gcol, float* s) {
-    if (p.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint4 b8 = *reinterpret_cast<const uint4*>(p.bias + gcol + 8 * j);
-            const uint32_t w[4] = {b8.x, b8.y, b8.z, b8.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                s[8 * j + 2 * e] = __fadd_rn(s[8 * j + 2 * e], f.x);
-                s[8 * j + 2 * e + 1] = __fadd_rn(s[8 * j + 2 * e + 1], f.y);
-            }
-        }
-    }
-    if (p.activation == kActRelu) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fmaxf(s[i], 0.f);
-    } else if (p.activation == kActSilu) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = __fdividef(s[i], 1.f + __expf(-s[i]));
-    }
-}
-
-// The residual's COLS columns (a multiple of 8) of one row from gcol on: requested together, ahead of the arithmetic
-// that they are added behind.
-template <int COLS>
-__device__ __forceinline__ void load_residual(const GemmParams& p, int l, long long row, int gcol, uint4 (&r)[COLS / 8]) {
-    const __half* src = p.residual + l * p.residual_batch_stride + row * p.residual_row_stride + gcol;
-#pragma unroll
-    for (int j = 0; j < COLS / 8; ++j) r[j] = *reinterpret_cast<const uint4*>(src + 8 * j);
-}
-// s[0..15] += sixteen fp16 of the residual
-__device__ __forceinline__ void add_residual16(const uint4 (&r)[2], float* s) {
+// s[0..15] += sixteen fp16
+__device__ __forceinline__ void add_fp16x16(const uint4 (&r)[2], float* s) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
@@ -308,7 +282,32 @@ __device__ __forceinline__ void add_residual16(const uint4 (&r)[2], float* s) {
         }
     }
 }
+__device__ __forceinline__ void activate16(int activation, float* s) {
+    if (activation == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fmaxf(s[i], 0.f);
+    } else if (activation == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __fdividef(s[i], 1.f + __expf(-s[i]));
+    }
+}
+// bias and activation on 16 columns from output column gcol on (extended epilogue)
+__device__ __forceinline__ void bias_act16(const GemmParams& p, int gcol, float* s) {
+    if (p.bias != nullptr) {
+        const uint4 b[2] = {*reinterpret_cast<const uint4*>(p.bias + gcol), *reinterpret_cast<const uint4*>(p.bias + gcol + 8)};
+        add_fp16x16(b, s);
+    }
+    activate16(p.activation, s);
+}
 
+// The residual's COLS columns (a multiple of 8) of one row from gcol on: requested together, ahead of the arithmetic
+// that they are added behind.
+template <int COLS>
+__device__ __forceinline__ void load_residual(const GemmParams& p, int l, long long row, int gcol, uint4 (&r)[COLS / 8]) {
+    const __half* src = p.residual + l * p.residual_batch_stride + row * p.residual_row_stride + gcol;
+#pragma unroll
+    for (int j = 0; j < COLS / 8; ++j) r[j] = *reinterpret_cast<const uint4*>(src + 8 * j);
+}
 // At the end of a CTA whose wait ran out: longer than a copy into shared memory that is on its way can take.
 __device__ __forceinline__ void let_copies_land() {
     constexpr long long kCycles = 40000;          // 20 us at the highest clock; a copy takes one or two
@@ -353,9 +352,9 @@ __device__ __forceinline__ void leave_cluster(bool gave_up) {
 }
 
 template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int KS = 1, int EPI_EX = kEpiPlain, int EPI_WARPS = 0>
-__global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS>::kThreads, 1) gemm_nvfp4_kernel(const __grid_constant__ GemmParams p) {
-    static_assert(!(EPI_EX && TMA_STORE), "the extended epilogue writes with plain stores");
-    using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS>;
+__global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS, EPI_EX == kEpiResidualFp16>::kThreads, 1) gemm_nvfp4_kernel(const __grid_constant__ GemmParams p) {
+    static_assert((EPI_EX == kEpiResidualFp16) == TMA_STORE || EPI_EX == kEpiPlain, "which epilogues write with tensor stores");
+    using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS, EPI_WARPS, EPI_EX == kEpiResidualFp16>;
     constexpr int kNumAcc = S::kNumAcc;
     constexpr bool kAccOverlap = S::kAccOverlap;
     constexpr int kSfaCol = kAccOverlap ? kSfaColOverlap : kSfaColPlain;
@@ -381,7 +380,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
     const uint32_t bar_acc_full = bar_empty + STAGES * 8;
     const uint32_t bar_acc_empty = bar_acc_full + 2 * 8;
     const uint32_t bar_fix_full = bar_acc_empty + 2 * 8;
-    const uint32_t tmem_slot = bar_fix_full + S::kFixBufs * 8;
+    const uint32_t tmem_slot = smem_base + S::kBarOff + S::kNumBars * 8;
     volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(smem_gen + S::kBarOff + S::kNumBars * 8);
     volatile uint32_t* abort_flag = tmem_slot_gen + 1;
 
@@ -407,6 +406,8 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
             ptx::mbar_init(bar_acc_full + a * 8, 1);
             ptx::mbar_init(bar_acc_empty + a * 8, S::kEpiWarps * CG);
         }
+        if constexpr (EPI_EX == kEpiResidualFp16)
+            for (int w = 0; w < S::kEpiWarps; ++w) ptx::mbar_init(bar_fix_full + (S::kFixBufs + w) * 8, 1);
         *abort_flag = 0u;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&p.tma_a);
@@ -414,6 +415,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
         ptx::prefetch_tensormap(&p.tma_sfa);
         ptx::prefetch_tensormap(&p.tma_sfb);
         if (TMA_STORE) ptx::prefetch_tensormap(&p.tma_c);
+        if (EPI_EX == kEpiResidualFp16) ptx::prefetch_tensormap(&p.tma_res);
         if (TMA_STORE && p.peer_tma)
             for (int r = 0; r < p.n_peer; ++r) ptx::prefetch_tensormap(&p.tma_c_peer[r]);
     }
@@ -637,6 +639,13 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
         const int group = (warp - 2) / 4;      // which share of a tile's columns
         uint32_t acc_it = 0;
         uint32_t store_buf = 0;
+        // (residual) this warp's staging buffers, one for every 64 columns of its share, and the barrier on which they fill
+        [[maybe_unused]] const uint32_t staging = smem_base + S::kEpiOff + (warp - 2) * S::kStagingPerWarp;
+        [[maybe_unused]] const uint32_t bias_smem = smem_base + S::kBiasOff + (warp - 2) * S::kBiasPerWarp;
+        [[maybe_unused]] const uint32_t bar_res = bar_fix_full + S::kFixBufs * 8 + (warp - 2) * 8;
+        [[maybe_unused]] const uint64_t pol_res = EPI_EX == kEpiResidualFp16 ? ptx::policy_evict_first() : 0;
+        [[maybe_unused]] uint32_t res_phase = 0;
+        static_assert(EPI_EX != kEpiResidualFp16 || S::kStagingBufs == kMyChunks / 2, "a staging buffer for every 64 columns of a warp's share");
         // NVFP4 output: whether 32-byte code stores and 4-byte scale stores are aligned
         const bool wide_packed = EPI_EX && ((reinterpret_cast<uintptr_t>(p.out_packed) | static_cast<uintptr_t>(p.out_packed_row_stride) |
                                               static_cast<uintptr_t>(p.out_packed_batch_stride)) & 31u) == 0;
@@ -653,11 +662,35 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
             const int l = tc.l;
             const uint32_t acc = acc_it % kNumAcc;
             const uint32_t acc_phase = (acc_it / kNumAcc) & 1u;
+            // With a residual: this warp's share of the tile is on its way into its staging buffers while the accumulator is
+            // still being made; the sums replace it there and leave by tensor stores.  (Read by the lanes instead, each along its own row, 4096 x
+            // 7168 x 7168 took 111-117 us; loads of the epilogue's compete with the operands' in the path from L2.)
+            if constexpr (EPI_EX == kEpiResidualFp16) {
+                if (k0 == 0 && lane == 0) {
+                    ptx::bulk_wait_group_read<0>();      // the previous tile's stores have left the buffers
+                    ptx::mbar_expect_tx(bar_res, kMyChunks / 2 * (4096 + (p.bias ? 128 : 0)));
+                    const int first = (kAccOverlap && (acc_it % kNumAcc) == 0) ? kChunks / 2 : 0;
+#pragma unroll
+                    for (int ci = 0; ci < kMyChunks / 2; ++ci) {
+                        const int at = 2 * ci < kMyRelease ? group * kMyRelease + 2 * ci : kReleaseAfter + group * (kMyChunks - kMyRelease) + (2 * ci - kMyRelease);
+                        const int col = nb * BN + ((at + first) & (kChunks - 1)) * 32;
+                        ptx::tma_load_3d(staging + ci * 4096, &p.tma_res, col, mb * kBM + quad * 32, l, bar_res, pol_res);
+                        if (p.bias) ptx::bulk_load(bias_smem + ci * 128, p.bias + col, 128, bar_res);
+                    }
+                }
+                __syncwarp();
+            }
             // All epilogue threads take the same branch: the outcome of the wait is agreed on
             // through a barrier, so a thread that gave up cannot strand the others at a later one.
             // One warp polls; the others sleep in the barrier below (a polling warp costs power, and with it clock).
             bool got_acc = true;
             if (warp == 2) got_acc = ptx::mbar_wait_bounded(bar_acc_full + acc * 8, acc_phase, abort_flag, timeout);
+            if constexpr (EPI_EX == kEpiResidualFp16) {
+                if (k0 == 0) {
+                    got_acc = ptx::mbar_wait_bounded(bar_res, res_phase, abort_flag, timeout) && got_acc;
+                    res_phase ^= 1u;
+                }
+            }
             if (!ptx::named_bar_and(2, kEpiThreads, got_acc)) break;
             ptx::tc_fence_after();
             const uint32_t t_acc = tmem_base + acc * S::kAccStride + (static_cast<uint32_t>(quad * 32) << 16);
@@ -691,8 +724,8 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     // once.  Codes and scales of the NVFP4 form are collected and stored together: 64
                     // columns are 32 bytes of codes (one full sector) and the four scales of one unit of either layout.
                     const int gcol = nb * BN + c0;
-                    [[maybe_unused]] uint4 res[EPI_EX == kEpiResidual ? kCols / 8 : 2];
-                    if constexpr (EPI_EX == kEpiResidual) load_residual<kCols>(p, l, row, gcol, res);
+                    [[maybe_unused]] uint4 res[kHasResidual<EPI_EX> ? kCols / 8 : 2];
+                    if constexpr (kHasResidual<EPI_EX>) load_residual<kCols>(p, l, row, gcol, res);
                     uint32_t q[kCols / 8];
                     uint32_t sf = 0u;
 #pragma unroll
@@ -700,13 +733,13 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
 #pragma unroll 1
                     for (int h = 0; h < kCols; h += 16) {
                         bias_act16(p, gcol + h, s);
-                        if constexpr (EPI_EX == kEpiResidual) {
+                        if constexpr (kHasResidual<EPI_EX>) {
                             const uint4 now[2] = {res[0], res[1]};
-                            add_residual16(now, s);
+                            add_fp16x16(now, s);
 #pragma unroll
                             for (int j = 0; j + 2 < kCols / 8; ++j) res[j] = res[j + 2];
                         }
-                        if (!p.out_nvfp4) {
+                        if (EPI_EX == kEpiResidualFp16 || !p.out_nvfp4) {
                             store8(c0 + h, pack8_fp16(&s[0]));
                             store8(c0 + h + 8, pack8_fp16(&s[8]));
                         } else {
@@ -727,7 +760,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
 #pragma unroll
                         for (int i = 0; i + 16 < kCols; ++i) s[i] = s[i + 16];
                     }
-                    if (p.out_nvfp4) {
+                    if (EPI_EX != kEpiResidualFp16 && p.out_nvfp4) {
                         const int blk = gcol / 16;
                         uint8_t* dst = p.out_packed + l * p.out_packed_batch_stride + static_cast<long long>(row) * p.out_packed_row_stride + gcol / 2;
                         uint8_t* sf_plain = p.out_sf + l * p.out_sf_batch_stride + static_cast<long long>(row) * p.out_sf_row_stride + blk;
@@ -767,6 +800,23 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     if (CG == 2 && !leader) ptx::mbar_arrive_cluster_signal(bar, 0);
                     else ptx::mbar_arrive(bar);
                 }
+            };
+
+            // Waits until the other workers have published `need` k-tiles of a shared tile.
+            [[maybe_unused]] auto wait_for_others = [&](int* counter, int need) {
+                bool ready = true;
+                if (epi_tid == 0) {
+                    const long long t_spin = clock64();
+                    while (ptx::ld_acquire_gpu(counter) < need) {
+                        if (*abort_flag || static_cast<uint64_t>(clock64() - t_spin) > timeout) {
+                            *abort_flag = 1u;
+                            ready = false;
+                            break;
+                        }
+                        __nanosleep(64);
+                    }
+                }
+                return ptx::named_bar_and(1, kEpiThreads, ready);
             };
 
             if constexpr (KS > 1) {
@@ -905,7 +955,70 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     if (row < p.M) emit(ks_rank * kMyCols + c0, s);
                 }
                 release_acc();
-            } else if (TMA_STORE && whole_tile) {
+            } else if (EPI_EX == kEpiResidualFp16 && k0 == 0) {
+                if constexpr (EPI_EX == kEpiResidualFp16) {
+                    // The piece that the other accumulator shares goes to registers and is handed back first; then 64 columns at a
+                    // time: partial sums of the other workers (a shared tile), bias, activation, residual, and out.
+                    uint8_t* const staging_gen = smem_gen + S::kEpiOff + (warp - 2) * S::kStagingPerWarp;
+                    uint32_t held[kMyRelease][32];
+#pragma unroll
+                    for (int i = 0; i < kMyRelease; ++i) ptx::tc_ld_32cols(t_acc + my_chunk(i) * 32, held[i]);
+                    ptx::tc_wait_ld();
+                    release_acc();
+                    const int w_last = whole_tile ? worker : unit_owner(tile * KT + KT - 1, n_workers, p.total_units);
+                    if (!whole_tile && !wait_for_others(p.counters + worker * CG + cta_rank, KT - (k1 - k0))) break;
+                    auto finish = [&](int ci, const uint32_t (&lo)[32], const uint32_t (&hi)[32]) {
+                        const int c0 = my_chunk(2 * ci) * 32;
+                        float s[64];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) { s[e] = __uint_as_float(lo[e]); s[32 + e] = __uint_as_float(hi[e]); }
+#pragma unroll 1
+                        for (int w = worker + 1; w <= w_last; ++w) {
+                            const float* src = p.scratch + static_cast<long long>(partial_slot(w, 1, CG, cta_rank)) * (kBM * BN) + row_in_tile * 4;
+                            float4 t[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) t[j] = ptx::ld_cg_v4(src + (c0 / 4 + j) * (kBM * 4));
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                s[4 * j] += t[j].x; s[4 * j + 1] += t[j].y; s[4 * j + 2] += t[j].z; s[4 * j + 3] += t[j].w;
+                            }
+                        }
+                        uint8_t* const buf = staging_gen + ci * 4096 + lane * 128;     // this thread's row, 16-byte pieces, 128-byte swizzle
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            if (p.bias) {
+                                const uint4* b = reinterpret_cast<const uint4*>(smem_gen + S::kBiasOff + (warp - 2) * S::kBiasPerWarp + ci * 128 + h * 32);
+                                const uint4 now[2] = {b[0], b[1]};
+                                add_fp16x16(now, &s[16 * h]);
+                            }
+                            activate16(p.activation, &s[16 * h]);
+                            uint4* const at0 = reinterpret_cast<uint4*>(buf + (((2 * h) ^ (lane & 7)) << 4));
+                            uint4* const at1 = reinterpret_cast<uint4*>(buf + (((2 * h + 1) ^ (lane & 7)) << 4));
+                            const uint4 res[2] = {*at0, *at1};
+                            add_fp16x16(res, &s[16 * h]);
+                            *at0 = pack8_fp16(&s[16 * h]);
+                            *at1 = pack8_fp16(&s[16 * h + 8]);
+                        }
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0 && mb * kBM + quad * 32 < p.M) {
+                            ptx::tma_store_3d(&p.tma_c, staging + ci * 4096, nb * BN + c0, mb * kBM + quad * 32, l);
+                            ptx::bulk_commit_group();
+                        }
+                    };
+#pragma unroll
+                    for (int ci = 0; ci < kMyRelease / 2; ++ci) finish(ci, held[2 * ci], held[2 * ci + 1]);
+#pragma unroll 1
+                    for (int ci = kMyRelease / 2; ci < kMyChunks / 2; ++ci) {
+                        uint32_t lo[32], hi[32];
+                        ptx::tc_ld_32cols(t_acc + my_chunk(2 * ci) * 32, lo);
+                        ptx::tc_ld_32cols(t_acc + my_chunk(2 * ci + 1) * 32, hi);
+                        ptx::tc_wait_ld();
+                        finish(ci, lo, hi);
+                    }
+                    if (!whole_tile && epi_tid == 0) p.counters[worker * CG + cta_rank] = 0;
+                }
+            } else if (TMA_STORE && EPI_EX == kEpiPlain && whole_tile) {
                 if constexpr (TMA_STORE) {
                     // 64 columns (128 bytes of fp16) at a time through a swizzled 32-row staging buffer.
                     uint8_t* staging_gen = smem_gen + S::kEpiOff + (warp - 2) * S::kStagingPerWarp;
@@ -1021,7 +1134,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     __threadfence();
                     ptx::named_bar_sync(1, kEpiThreads);
                     if (epi_tid == 0) atomicAdd(counter, k1 - k0);
-                } else {
+                } else if constexpr (EPI_EX != kEpiResidualFp16) {
                     // Finish: the rest of the k-range has been published (normally long ago); add
                     // those partials, read straight from L2, to this worker's accumulator in
                     // ascending worker order.  The operand ring keeps this SM's path from L2 busy,
@@ -1035,21 +1148,6 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     // kernel than after itself.)  What the hand-back waits for is the first step's: it goes to
                     // registers, the accumulator is released, and only then anything is waited for, converted or
                     // stored; one group of warps over 256 columns (plain stores of little code) holds two steps.
-                    auto wait_for_others = [&]() {
-                        bool ready = true;
-                        if (epi_tid == 0) {
-                            const long long t_spin = clock64();
-                            while (ptx::ld_acquire_gpu(counter) < need) {
-                                if (*abort_flag || static_cast<uint64_t>(clock64() - t_spin) > timeout) {
-                                    *abort_flag = 1u;
-                                    ready = false;
-                                    break;
-                                }
-                                __nanosleep(64);
-                            }
-                        }
-                        return ptx::named_bar_and(1, kEpiThreads, ready);
-                    };
                     auto finish64 = [&](int c0, float (&s)[64]) {       // own sums in, total out
 #pragma unroll 1
                         for (int w = w_first + 1; w <= w_last; ++w) {   // later contributors use their "head" slot
@@ -1072,7 +1170,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                         for (int i = 0; i < 4; ++i) ptx::tc_ld_32cols(t_acc + my_chunk(i) * 32, held[i]);
                         ptx::tc_wait_ld();
                         release_acc();
-                        if (!whole_tile && !wait_for_others()) break;
+                        if (!whole_tile && !wait_for_others(counter, need)) break;
 #pragma unroll
                         for (int i = 0; i < 4; i += 2) {
                             float s[64];
@@ -1095,7 +1193,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                         }
                         if (kMyRelease == 2 && i == 0) {
                             release_acc();
-                            if (!whole_tile) ready = wait_for_others();
+                            if (!whole_tile) ready = wait_for_others(counter, need);
                             if (!ready) break;
                         }
                         finish64(c0, s);

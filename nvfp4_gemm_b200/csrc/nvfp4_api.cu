@@ -233,7 +233,7 @@ WorkSplit plan_work_split(long long tiles, int k_tiles, int max_workers, double 
 template <int CG, int BN, int STAGES, bool TMA_STORE, int EPI_KB, int EPI_EX = kEpiPlain, int EPI_WARPS = 0>
 int launch_gemm(DeviceCtx* c, int variant, GemmParams& params, const nvfp4_gemm_config& cf, cudaStream_t stream, const char* name) {
     const int grid_request = cf.grid;
-    using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, 1, EPI_WARPS>;
+    using S = GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, 1, EPI_WARPS, EPI_EX == kEpiResidualFp16>;
     auto kernel = gemm_nvfp4_kernel<CG, BN, STAGES, TMA_STORE, EPI_KB, 1, EPI_EX, EPI_WARPS>;
     if (!c->smem_attr_set[variant]) {
         CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kDynamicBytes));
@@ -283,7 +283,7 @@ int launch_gemm(DeviceCtx* c, int variant, GemmParams& params, const nvfp4_gemm_
         // from the groups beyond about 93 MB only (to NVFP4: 4096 x 4096 x 7168 x 4 271 -> 204 us, 4096 x 2560 x 7168 x 4, 95 MB,
         // 164 -> 145; 2304 x 4096 x 7168 x 4, 92 MB, 119 -> 128, 3000 x 7168 x 4096 x 4, 83 MB, 228 -> 252).
         const double operand_bytes = static_cast<double>(params.L) * (static_cast<double>(params.M) + params.N) * (params.K / 2);
-        if (split.whole_tiles && cf.raster == 0 && (params.tiles_m < 8 || params.tiles_n < 4 || (EPI_EX && operand_bytes < 93e6))) params.raster_rows = 0;
+        if (split.whole_tiles && cf.raster == 0 && (params.tiles_m < 8 || params.tiles_n < 4 || (EPI_EX && !TMA_STORE && operand_bytes < 93e6))) params.raster_rows = 0;
     }
     params.order_k = params.whole_tiles ? 1 : params.k_tiles;
     params.order_total = params.whole_tiles ? params.total_units / params.k_tiles : params.total_units;
@@ -632,7 +632,10 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
     // Whole tiles leave through the TMA-store epilogue unless the caller asks for plain stores.
     int epilogue = cf.epilogue;
     if (epilogue == 0) epilogue = 2;
-    if (epi) epilogue = 1;                     // the extended epilogue writes with plain stores
+    // The extended epilogue writes with plain stores; with a residual, fp16 leaves by tensor stores and the residual comes by tensor loads,
+    // where its rows can be described to them and its tile fits beside the operands' ring.
+    const bool residual_tma = residual && !to_nvfp4 && residual->row_stride >= p->n && (p->l == 1 || residual->batch_stride >= p->n) && !(cg == 1 && bn == 256);
+    if (epi) epilogue = residual_tma ? 2 : 1;
     const uint64_t kbytes = static_cast<uint64_t>(p->k) / 2;
     const uint64_t a_bs = p->l > 1 ? static_cast<uint64_t>(p->a_batch_stride) : static_cast<uint64_t>(p->a_row_stride) * p->m;
     const uint64_t b_bs = p->l > 1 ? static_cast<uint64_t>(p->b_batch_stride) : static_cast<uint64_t>(p->b_row_stride) * p->n;
@@ -656,6 +659,13 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
                                                  CU_TENSOR_MAP_DATA_TYPE_FLOAT16),
                                      &g.tma_c_peer[i])) return rc;
         }
+    }
+
+    if (residual_tma) {
+        const uint64_t r_bs = p->l > 1 ? static_cast<uint64_t>(residual->batch_stride) * 2 : static_cast<uint64_t>(residual->row_stride) * 2 * p->m;
+        if (int rc = encode_map(make_key(residual->ptr, p->n, p->m, p->l, static_cast<uint64_t>(residual->row_stride) * 2, r_bs, 64, 32,
+                                         CU_TENSOR_MAP_DATA_TYPE_FLOAT16),
+                             &g.tma_res)) return rc;
     }
 
     const DecodeChoice decode = choose_decode(p->m, p->n, p->k, p->l, c->num_sms, cf);
@@ -706,6 +716,11 @@ int gemm_impl(const nvfp4_problem* p, const nvfp4_gemm_config* cfg, const nvfp4_
         return launch_gemm_splitk<256, 4, 0, 8>(c, 11, g, stream, "gemm_splitk8_n256_s4");
     }
 
+    if (residual_tma) {
+        if (cg == 2 && bn == 256) return launch_gemm<2, 256, 4, true, 64, kEpiResidualFp16, 8>(c, 27, g, cf, stream, "gemm_2cta_n256_s4_residual_tmastore");
+        if (cg == 2) return launch_gemm<2, 128, 6, true, 32, kEpiResidualFp16>(c, 28, g, cf, stream, "gemm_2cta_n128_s6_residual_tmastore");
+        return launch_gemm<1, 128, 5, true, 32, kEpiResidualFp16>(c, 29, g, cf, stream, "gemm_1cta_n128_s5_residual_tmastore");
+    }
     if (residual) {
         if (cg == 2 && bn == 256) return launch_gemm<2, 256, 5, false, 32, kEpiResidual>(c, 23, g, cf, stream, "gemm_2cta_n256_s5_residual");
         if (cg == 2) return launch_gemm<2, 128, 6, false, 32, kEpiResidual>(c, 24, g, cf, stream, "gemm_2cta_n128_s6_residual");

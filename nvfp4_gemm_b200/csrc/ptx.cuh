@@ -184,6 +184,11 @@ __device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar_cluster_addr)
         : "memory");
 }
+// Untiled copy global -> shared memory (both addresses and the size multiples of 16), signalled on an mbarrier of this CTA.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // Bulk copy from this CTA's shared memory into another CTA's of the cluster (both addresses and
 // the size multiples of 16); the bytes are signalled on an mbarrier of the destination CTA.
 // dst and bar are shared::cluster addresses (mapa).
