@@ -45,9 +45,12 @@ struct ExpertGemmParams {
     long long out_packed_row_stride;   // bytes
     uint8_t* out_sf;                   // atoms, tile after tile like the input's
     int n, n_out, k_tiles, tiles_n;
+    int experts, most_tiles;  // bounds of what the tables hold
     int* status;
     unsigned long long timeout_cycles;
 };
+
+constexpr int kExpertPrefetch = 4;   // k-tiles of a CTA's first tile prefetched ahead of the dependency wait
 
 template <int CG, int BT, int STAGES, int EPI_WARPS>
 struct ExpertSmem {
@@ -85,11 +88,11 @@ struct ExpertTiles {
     int tiles_n, idx, total, step;
     int4 ahead;
     __device__ ExpertTiles(const ExpertGemmParams& p, int worker, int workers)
-        : tiles(p.tiles), tiles_n(p.tiles_n), idx(worker - workers), total(*p.tile_count * p.tiles_n), step(workers) {
+        : tiles(p.tiles), tiles_n(p.tiles_n), idx(worker - workers), total(__ldcg(p.tile_count) * p.tiles_n), step(workers) {
         look_ahead(worker);
     }
     __device__ __forceinline__ void look_ahead(int i) {
-        if (i < total) ahead = tiles[i / tiles_n];
+        if (i < total) ahead = __ldcg(&tiles[i / tiles_n]);
     }
     // the next tile: its entry, which token tile and which block it is
     __device__ __forceinline__ bool next(int4* t, int* tt, int* nt) {
@@ -147,16 +150,34 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
         ptx::tmem_relinquish<CG>();
         ptx::tc_fence_before();
     }
-    ptx::grid_dependency_launch_dependents();
+    const int KT = p.k_tiles;
+    const int worker = static_cast<int>(blockIdx.x) / CG, workers = static_cast<int>(gridDim.x) / CG;
+    // The weights of this CTA's first tile are asked into L2 ahead of the dependency wait: the router is usually done by now, only the kernel
+    // that quantises the rows is not.  What stands in the table may still change (it may even be another call's left-overs): nothing
+    // but a prefetch is made of it, and it is read past L1, so that what is read after the wait is read anew.
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            const int count = min(__ldcg(p.tile_count), p.most_tiles);
+            if (worker < count * p.tiles_n) {
+                const int expert = __ldcg(&p.tiles[worker / p.tiles_n].x);
+                const int wb = (worker % p.tiles_n) * CG + cta_rank;
+                if (expert >= 0 && expert < p.experts)
+                    for (int kt = 0; kt < min(kExpertPrefetch, KT); ++kt) {
+                        ptx::tma_prefetch_3d(&p.tma_w, kt * kBKBytes, wb * kBM, expert);
+                        ptx::tma_prefetch_4d(&p.tma_sfw, 0, kt * kMmaPerStage, wb, expert);
+                    }
+            }
+        }
+        __syncwarp();
+    }
     ptx::grid_dependency_wait();
+    ptx::grid_dependency_launch_dependents();     // (behind the wait: see the prefetch above, of the kernel that follows)
     uint32_t tmem_base = 0;
     if (warp != 0) {
         ptx::named_bar_sync(3, S::kThreads - 32);
         ptx::tc_fence_after();
         tmem_base = *tmem_slot_gen;
     }
-    const int KT = p.k_tiles;
-    const int worker = static_cast<int>(blockIdx.x) / CG, workers = static_cast<int>(gridDim.x) / CG;
     const uint64_t timeout = p.timeout_cycles;
     // rows of a tile -> columns of its MMAs
     auto mma_n = [](int rows) { return CG == 2 ? (rows + 31) & ~31 : (rows + 15) & ~15; };

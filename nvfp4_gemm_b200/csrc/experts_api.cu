@@ -351,6 +351,8 @@ int nvfp4_expert_gemm(const nvfp4_expert_problem* p, const nvfp4_routing* r, voi
         g.c_row_stride = p->out_row_stride;
     }
     g.n = p->n; g.n_out = n_out;
+    g.experts = r->experts;
+    g.most_tiles = static_cast<int>(s.max_tiles);
     g.k_tiles = p->k / kKPerStage;
     g.status = c->status_dev;
     g.timeout_cycles = g_timeout_ns.load() * 2;   // SM clock <= 2 GHz: at least the requested time

@@ -712,8 +712,8 @@ __global__ void __launch_bounds__(256) quantize_routed_kernel(const QuantizeRout
     const long long unit = static_cast<long long>(blockIdx.x) * 8 + warp;
     const long long token = unit / col_units;
     const int blk = static_cast<int>(unit - token * col_units) * (kRoutedCols / 16) + lane;
-    ptx::grid_dependency_launch_dependents();
     ptx::grid_dependency_wait();
+    ptx::grid_dependency_launch_dependents();     // (behind the wait: the product that follows looks at the routing's tables ahead of its own)
     if (token >= p.tokens) return;
     const bool in_row = blk < blocks;
     int row = -1, sf_row = -1;
