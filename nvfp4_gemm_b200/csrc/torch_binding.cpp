@@ -279,6 +279,26 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 // What a call makes itself, on the device of `on`.
 at::Tensor fresh(const at::Tensor& on, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, on.options().dtype(type)); }
 
+// Several results in one allocation (each costs the caching allocator more than a small kernel's launch leaves room for): tensors
+// of their own on one storage, which lives as long as any of them.
+class Slab {
+public:
+    Slab(const at::Tensor& on, int64_t bytes) : base_(at::empty({bytes}, on.options().dtype(at::kByte).requires_grad(false))) {}
+    static int64_t room(int64_t bytes) { return (bytes + 255) & ~int64_t{255}; }
+    at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
+        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(), c10::scalarTypeToTypeMeta(type));
+        const int64_t item = static_cast<int64_t>(c10::elementSize(type));
+        impl->set_storage_offset(used_ / item);
+        impl->set_sizes_contiguous(sizes);
+        used_ += room(c10::multiply_integers(sizes) * item);
+        return at::Tensor(std::move(impl));
+    }
+
+private:
+    at::Tensor base_;
+    int64_t used_ = 0;
+};
+
 PyObject* status_object(int rc) { return PyLong_FromLong(rc); }
 
 PyObject* pack(std::initializer_list<at::Tensor> tensors) {
@@ -302,14 +322,22 @@ struct Routing {
     int64_t sf_rows = 0;
     at::Tensor row, offset, plan;
     int status;
-    // new rows, offsets and plan for [tokens, top_k] choices
-    Routing(const at::Tensor& on, int64_t tokens, int64_t top_k, int64_t experts) {
+    at::Tensor expert, weight;
+    // new rows, offsets and plan for [tokens, top_k] choices, and the choices and their weights too (choose)
+    Routing(const at::Tensor& on, int64_t tokens, int64_t top_k, int64_t experts, bool choose) {
         int64_t plan_bytes = 0;
         status = size(tokens, top_k, experts, &plan_bytes);
         if (status) return;
-        row = fresh(on, {tokens, top_k}, at::kInt);
-        offset = fresh(on, {experts + 1}, at::kInt);
-        plan = fresh(on, {plan_bytes / 4}, at::kInt);
+        const int64_t per_pair = Slab::room(tokens * top_k * 4);
+        Slab slab(on, per_pair * (choose ? 3 : 1) + Slab::room((experts + 1) * 4) + Slab::room(plan_bytes));
+        row = slab.take({tokens, top_k}, at::kInt);
+        offset = slab.take({experts + 1}, at::kInt);
+        plan = slab.take({plan_bytes / 4}, at::kInt);
+        if (choose) {
+            expert = slab.take({tokens, top_k}, at::kInt);
+            weight = slab.take({tokens, top_k}, at::kFloat);
+            r.expert = expert.data_ptr<int32_t>();
+        }
         r.row = row.data_ptr<int32_t>();
         r.offset = offset.data_ptr<int32_t>();
         r.plan = plan.data_ptr();
@@ -375,15 +403,13 @@ PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         o.renormalize = int_arg(args[7]);
         o.scale = static_cast<float>(float_arg(args[8]));
         const c10::cuda::CUDAGuard guard(logits.device());
-        Routing routing(logits, logits.size(0), top_k, logits.size(1));
+        Routing routing(logits, logits.size(0), top_k, logits.size(1), true);
         if (routing.status) return status_object(routing.status);
-        const at::Tensor experts = fresh(logits, {logits.size(0), top_k}, at::kInt), weights = fresh(logits, {logits.size(0), top_k}, at::kFloat);
-        routing.r.expert = experts.data_ptr<int32_t>();
         o.logits = logits.data_ptr();
         o.logits_row_stride = row_stride(logits);
-        o.weights = weights.data_ptr<float>();
+        o.weights = routing.weight.data_ptr<float>();
         const int rc = on_current_stream(logits, [&](void* stream) { return nvfp4_route(&o, &routing.r, stream); });
-        return rc ? status_object(rc) : pack({experts, weights, routing.row, routing.offset, routing.plan});
+        return rc ? status_object(rc) : pack({routing.expert, routing.weight, routing.row, routing.offset, routing.plan});
     });
 }
 
@@ -396,7 +422,7 @@ PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (experts.dim() != 2 || experts.scalar_type() != at::kInt || !experts.is_contiguous())
             raise(PyExc_ValueError, "experts must be a contiguous int32 tensor [tokens, top_k]");
         const c10::cuda::CUDAGuard guard(experts.device());
-        Routing routing(experts, experts.size(0), experts.size(1), int_arg(args[1]));
+        Routing routing(experts, experts.size(0), experts.size(1), int_arg(args[1]), false);
         if (routing.status) return status_object(routing.status);
         routing.r.expert = experts.data_ptr<int32_t>();
         const int rc = on_current_stream(experts, [&](void* stream) { return nvfp4_plan_experts(&routing.r, stream); });
@@ -417,8 +443,9 @@ PyObject* py_quantize_routed(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         if (routing.status) return status_object(routing.status);
         if (routing.r.tokens != x.size(0)) raise(PyExc_ValueError, "x must have a row per token of the routing");
         const int64_t k = size_arg(x.size(1), "the width of x");
-        const at::Tensor packed = fresh(x, {routing.row.numel(), k / 2}, at::kFloat4_e2m1fn_x2);
-        const at::Tensor sf = fresh(x, {routing.sf_rows * (k / 16)}, at::kFloat8_e4m3fn);
+        const int64_t rows = routing.row.numel();
+        Slab slab(x, Slab::room(rows * (k / 2)) + Slab::room(routing.sf_rows * (k / 16)));
+        const at::Tensor packed = slab.take({rows, k / 2}, at::kFloat4_e2m1fn_x2), sf = slab.take({routing.sf_rows * (k / 16)}, at::kFloat8_e4m3fn);
         const void* const src = x.data_ptr();
         void *const codes = packed.data_ptr(), *const scales = sf.data_ptr();
         const bool bf16 = x.scalar_type() == at::kBFloat16;
@@ -488,8 +515,9 @@ PyObject* py_expert_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         at::Tensor out, out_sf;
         if (to_nvfp4) {
             if (args[12] != Py_None) raise(PyExc_ValueError, "out is for the fp16 result");
-            out = fresh(a, {rows, n_out / 2}, at::kFloat4_e2m1fn_x2);
-            out_sf = fresh(a, {routing.sf_rows * (n_out / 16)}, at::kFloat8_e4m3fn);
+            Slab slab(a, Slab::room(rows * (n_out / 2)) + Slab::room(routing.sf_rows * (n_out / 16)));
+            out = slab.take({rows, n_out / 2}, at::kFloat4_e2m1fn_x2);
+            out_sf = slab.take({routing.sf_rows * (n_out / 16)}, at::kFloat8_e4m3fn);
             p.output = NVFP4_OUT_NVFP4;
             p.out_row_stride = n_out / 2;
             p.out_sf = out_sf.data_ptr();
