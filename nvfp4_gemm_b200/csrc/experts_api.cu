@@ -389,8 +389,9 @@ int nvfp4_combine_experts(const void* y, int64_t y_row_stride, int32_t y_rows, c
     const long long grid = (static_cast<long long>(tokens) * (n / 8) + 255) / 256;
     if (grid > 0x7fffffffll) return fail(NVFP4_ERR_INVALID_ARGUMENT, "problem too large: %lld CTAs", grid);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-    return out_is_bf16 ? launch(combine_kernel<true>, static_cast<unsigned>(grid), 256, 0, 1, stream, "combine_experts", p)
-                       : launch(combine_kernel<false>, static_cast<unsigned>(grid), 256, 0, 1, stream, "combine_experts", p);
+    auto go = [&](auto kernel) { return launch(kernel, static_cast<unsigned>(grid), 256, 0, 1, stream, "combine_experts", p); };
+    if (out_is_bf16) return top_k <= 2 ? go(combine_kernel<true, 2>) : top_k <= 4 ? go(combine_kernel<true, 4>) : go(combine_kernel<true, 8>);
+    return top_k <= 2 ? go(combine_kernel<false, 2>) : top_k <= 4 ? go(combine_kernel<false, 4>) : go(combine_kernel<false, 8>);
 }
 
 }  // extern "C"
