@@ -349,8 +349,8 @@ int nvfp4_route(const nvfp4_router* router, const nvfp4_routing* routing, void* 
 int nvfp4_plan_experts(const nvfp4_routing* routing, void* stream);
 
 /*
- * Token rows x (fp16, or bf16 if x_is_bf16; [tokens][k], 16-byte aligned, stride in elements a multiple of 8) -> NVFP4 rows in expert
- * order: packed [tokens * top_k][k / 2] and sf.  A token is quantised once, by the rule of nvfp4_quantize(), and
+ * Token rows x (fp16, or bf16 if x_is_bf16; [tokens][k], 16-byte aligned, stride in elements a multiple of 8, 0 for one row for all) -> NVFP4 rows in
+ * expert order: packed [tokens * top_k][k / 2] and sf.  A token is quantised once, by the rule of nvfp4_quantize(), and
  * written to each of its rows.  k a multiple of 64.
  */
 int nvfp4_quantize_routed(const void* x, int32_t x_is_bf16, int64_t x_row_stride, int32_t k, const nvfp4_routing* routing, void* packed,

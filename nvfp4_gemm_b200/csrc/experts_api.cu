@@ -31,10 +31,11 @@ int plan_sizes(int tokens, int top_k, int experts, PlanSizes* s) {
     s->max_tiles = pairs / s->tile_tokens + (pairs < experts ? pairs : experts);
     s->sf_rows = s->max_tiles * s->tile_sf_rows;
     if (pairs > 0x7fffffffll || s->sf_rows > 0x7fffffffll) return fail(NVFP4_ERR_INVALID_ARGUMENT, "problem too large: %lld pairs", pairs);
-    // Chunks of the tokens.  Up to 128 tokens are one: choice and order take one launch.  Else one CTA each, 148 at most
+    // Chunks of the tokens.  Up to 1024 pairs of up to 512 tokens are one: choice and order take one launch.  Else one CTA each, 148 at most
     // (more only where a chunk's pairs would not be counted in 16 bits).
-    constexpr int kUnit = 8, kMostChunks = 148, kOneChunk = 128;
-    int chunk_tokens = tokens <= kOneChunk ? kOneChunk : kUnit * ((tokens + kUnit * kMostChunks - 1) / (kUnit * kMostChunks));
+    constexpr int kUnit = 8, kMostChunks = 148, kOneChunk = 512, kOneChunkPairs = 1024;
+    const bool one = tokens <= kOneChunk && pairs <= kOneChunkPairs;
+    int chunk_tokens = one ? kOneChunk : kUnit * ((tokens + kUnit * kMostChunks - 1) / (kUnit * kMostChunks));
     if (chunk_tokens < 32) chunk_tokens = 32;
     if (chunk_tokens > kMaxChunkPairs / top_k) chunk_tokens = kMaxChunkPairs / top_k;
     s->chunk_tokens = chunk_tokens;
@@ -269,8 +270,8 @@ int nvfp4_quantize_routed(const void* x, int32_t x_is_bf16, int64_t x_row_stride
     if (int rc = check_routing(r, &s)) return rc;
     if (k < 64 || k % 64) return fail(NVFP4_ERR_INVALID_ARGUMENT, "k must be a positive multiple of 64 (got %d)", k);
     if (r->tokens > 0 && (!x || !packed || !sf || !r->row)) return fail(NVFP4_ERR_INVALID_ARGUMENT, "x, packed, sf and row must not be NULL");
-    if (!aligned(x, 16) || x_row_stride % 8 || (x_row_stride < k && r->tokens > 1))
-        return fail(NVFP4_ERR_INVALID_ARGUMENT, "x must be 16-byte aligned with a row stride (elements) that is a multiple of 8 and >= k");
+    if (!aligned(x, 16) || x_row_stride % 8 || x_row_stride < 0 || (x_row_stride < k && x_row_stride != 0 && r->tokens > 1))
+        return fail(NVFP4_ERR_INVALID_ARGUMENT, "x must be 16-byte aligned with a row stride (elements) that is a multiple of 8 and >= k, or 0");
     if (!aligned(packed, 8) || packed_row_stride % 8 || packed_row_stride < k / 2 || !aligned(sf, 16))
         return fail(NVFP4_ERR_INVALID_ARGUMENT, "packed must be 8-byte aligned with a row stride that is a multiple of 8 and >= k/2, sf 16-byte aligned");
     DeviceCtx* c = nullptr;

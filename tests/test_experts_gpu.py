@@ -408,3 +408,39 @@ def test_layers_on_two_streams_at_once(ex):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, exp[i]) for o in got[i])
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("experts,top_k", [(16, 3), (40, 4), (256, 8), (600, 32)])
+def test_equal_scores_go_to_the_lowest_experts(ex, lib, experts, top_k, bias):
+    """More equal keys than lanes, equal keys across the border of what is taken, and equal groups."""
+    x = torch.zeros((4, experts))
+    x[1, experts // 2:] = 1.0
+    x[2, ::3] = -2.0
+    x[3, experts - 1] = 5.0
+    kw = dict(bias=torch.zeros(experts)) if bias else dict()
+    for more in (dict(), dict(groups=4, top_groups=2), dict(groups=4, top_groups=2, group_score="top2")):
+        if experts % 4 or more.get("top_groups", 9) * experts // 4 < top_k:
+            continue
+        r = ex.route(x.cuda(), top_k, **{k: v.cuda() for k, v in kw.items()}, **more)
+        _check_routing(lib, r, x, top_k, experts, **kw, **more)
+
+
+def test_scores_at_the_border_of_what_32_bits_tell_apart(ex):
+    """Pairs of experts whose biased scores differ by 1e-9 .. 1e-7: in either order, among the taken and at the border, the 64-bit order decides."""
+    experts, top_k = 64, 4
+    g = _gen(11)
+    for scoring in ("sigmoid", "softmax"):
+        logits = torch.randn((200, experts), generator=g)
+        bias = torch.randn(experts, generator=g) * 0.1
+        s = torch.softmax(logits.double(), 1) if scoring == "softmax" else torch.sigmoid(logits.double())
+        # the bias of expert 1 makes its choice almost that of expert 0 in the first token, and so on: a bias per token, one call each
+        for t in range(0, 200, 8):
+            b = bias.double()
+            order = torch.argsort(s[t] + b, descending=True)
+            for a, c in ((0, 1), (top_k - 1, top_k), (2, 3)):
+                b[order[c]] += (s[t] + b)[order[a]] - (s[t] + b)[order[c]]
+            b32 = b.float()                                     # a rounding of 2^-25 or so: as near as it gets
+            exp, _ = ref.route(logits[t:t + 1], top_k, scoring=scoring, bias=b32)
+            r = ex.route(logits[t:t + 1].cuda(), top_k, scoring=scoring, bias=b32.cuda())
+            assert r.experts.cpu().tolist() == exp.tolist(), (scoring, t)
