@@ -311,7 +311,7 @@ typedef struct nvfp4_routing {
 /*
  * plan_bytes: size of nvfp4_routing.plan.  sf_rows: the scales of a routed operand (nvfp4_quantize_routed, the NVFP4 output of
  * nvfp4_expert_gemm) take sf_rows * (k / 16) bytes.  tile_tokens: rows of an expert that the grouped product takes
- * at a time (32, or 256 from 16 rows per expert on average).  Any of them may be NULL.
+ * at a time (32, or 256 from 20 rows per expert on average).  Any of them may be NULL.
  */
 int nvfp4_routing_plan(int32_t tokens, int32_t top_k, int32_t experts, int32_t* tile_tokens, int64_t* plan_bytes, int64_t* sf_rows);
 

@@ -45,7 +45,7 @@ struct ExpertGemmParams {
     long long out_packed_row_stride;   // bytes
     uint8_t* out_sf;                   // atoms, tile after tile like the input's
     int n, n_out, k_tiles, tiles_n;
-    int experts, most_tiles;  // bounds of what the tables hold
+    int experts, rows, most_tiles;     // bounds of what the tables hold
     int* status;
     unsigned long long timeout_cycles;
 };
@@ -83,12 +83,15 @@ struct ExpertSmem {
 
 // A worker's tiles: every workers-th of (token tile, block of weight rows).  The table entry of the next one is asked for
 // while the present one is worked on: read when it is needed it kept the MMA issuer waiting 500 cycles a tile.
+// What the table says is brought within the bounds of the operands (it is the plan's, but the plan's memory is the caller's).
+template <int BT>
 struct ExpertTiles {
     const int4* tiles;
-    int tiles_n, idx, total, step;
+    int tiles_n, idx, total, step, experts, rows;
     int4 ahead;
     __device__ ExpertTiles(const ExpertGemmParams& p, int worker, int workers)
-        : tiles(p.tiles), tiles_n(p.tiles_n), idx(worker - workers), total(__ldcg(p.tile_count) * p.tiles_n), step(workers) {
+        : tiles(p.tiles), tiles_n(p.tiles_n), idx(worker - workers), total(min(__ldcg(p.tile_count), p.most_tiles) * p.tiles_n), step(workers),
+          experts(p.experts), rows(p.rows) {
         look_ahead(worker);
     }
     __device__ __forceinline__ void look_ahead(int i) {
@@ -98,7 +101,9 @@ struct ExpertTiles {
     __device__ __forceinline__ bool next(int4* t, int* tt, int* nt) {
         idx += step;
         if (idx >= total) return false;
-        *t = ahead;
+        t->x = min(max(ahead.x, 0), experts - 1);
+        t->z = min(max(ahead.z, 1), min(BT, rows));
+        t->y = min(max(ahead.y, 0), rows - t->z);
         *tt = idx / tiles_n;
         *nt = idx - *tt * tiles_n;
         look_ahead(idx + step);
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
             const uint64_t pol_x = ptx::policy_evict_last();
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            ExpertTiles work(p, worker, workers);
+            ExpertTiles<BT> work(p, worker, workers);
             int4 t;
             int tt, nt;
             while (ok && work.next(&t, &tt, &nt)) {
@@ -236,7 +241,7 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
             if (ptx::elect_one()) {
                 uint32_t stage = 0, phase = 0, acc_it = 0, sf_buf = 0;
                 bool ok = true;
-                ExpertTiles work(p, worker, workers);
+                ExpertTiles<BT> work(p, worker, workers);
                 int4 t;
                 int tt, nt;
                 while (ok && work.next(&t, &tt, &nt)) {
@@ -292,7 +297,7 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
         uint8_t* const staging_gen = smem_gen + S::kEpiOff + (warp - 2) * S::kStagingPerWarp;
         const bool gated = p.activation == kExpertSwiglu;
         uint32_t acc_it = 0;
-        ExpertTiles work(p, worker, workers);
+        ExpertTiles<BT> work(p, worker, workers);
         int4 t;
         int tt, nt;
         while (work.next(&t, &tt, &nt)) {

@@ -699,6 +699,7 @@ struct QuantizeRoutedParams {
     const int* row;          // [tokens][top_k]
     const int* sf_row;
     int tokens, top_k, k;
+    int rows, sf_rows;       // bounds of what row and sf_row may say
     long long x_row_stride, packed_row_stride;   // bytes
 };
 
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(256) quantize_routed_kernel(const QuantizeRout
     scales |= __shfl_xor_sync(0xffffffffu, scales, 2);
     for (int j = 0; j < p.top_k; ++j) {
         const int r = __shfl_sync(0xffffffffu, row, j), s = __shfl_sync(0xffffffffu, sf_row, j);
-        if (r < 0 || !in_row) continue;
+        if (r < 0 || r >= p.rows || s < 0 || s >= p.sf_rows || !in_row) continue;
         *reinterpret_cast<uint2*>(p.packed + r * p.packed_row_stride + blk * 8) = make_uint2(codes[0], codes[1]);
         if ((lane & 3) == 0)
             *reinterpret_cast<uint32_t*>(p.sf + (static_cast<long long>(s / 128) * (blocks / 4) + blk / 4) * 512 + (s % 32) * 16 + (s % 128) / 32 * 4) = scales;
