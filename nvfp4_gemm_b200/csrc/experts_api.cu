@@ -134,6 +134,10 @@ template <bool BY_LOGIT, int VPL>
 int launch_route(DeviceCtx* c, int variant, RouteParams p, const PlanParams& q, cudaStream_t stream, const char* name) {
     // A warp per token.  Each has 128 words for candidates; with groups room for all keys, in 64 bits: at most 64 KB.
     constexpr int kMost = route_threads(VPL) / 32;
+    const int per = q.experts / p.groups, lanes = per / VPL;
+    p.direct_lanes = per % VPL == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    const size_t size = p.logit_type == kLogitFp32 ? 4 : 2, piece = VPL * size < 16 ? VPL * size : 16;
+    p.vector = aligned(p.logits, piece) && p.logits_row_stride * size % piece == 0;
     p.key_words = p.groups > 1 && 2 * q.experts > 128 ? (2 * q.experts + 3) & ~3 : 128;
     const int in_chunk = q.tokens < q.chunk_tokens ? q.tokens : q.chunk_tokens;
     // One chunk: up to eight CTAs, so that a scheduler has few tokens to issue for (32 tokens of 256 experts: 7.4 us, in one CTA 11.3).

@@ -33,6 +33,8 @@ struct RouteParams {
     int key_words;                 // shared memory of a warp, a multiple of 4
     int per_magic;                 // e * per_magic >> 20 is the group of expert e < 1024
     int group_lanes;               // lanes that judge a group: 32 / groups, rounded down to a power of two
+    int direct_lanes;              // lanes whose experts are just a group's (a power of two), or 0
+    int vector;                    // a lane's logits can be read in pieces of 16 bytes, or as much as it has
 };
 // Counts of a chunk: 16 bits an expert, whole 32-byte sectors.
 __host__ __device__ constexpr int counts_row(int experts) { return (experts + 15) & ~15; }
@@ -55,10 +57,11 @@ struct PlanParams {
 };
 
 // ------------------------------------------------------------------------------------------------ choice
-// Order-preserving unsigned keys; 0 is below every number.
+// Order-preserving unsigned keys.  0 is what cannot be chosen: the 32-bit keys are counted from that of -inf.
+constexpr uint32_t kLowestKey = 0x007fffffu;
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);   // (-0 becomes +0)
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (b & 0x80000000u ? ~b : b | 0x80000000u) - kLowestKey;
 }
 __device__ __forceinline__ uint64_t key_of(double v) {
     const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
@@ -67,7 +70,10 @@ __device__ __forceinline__ uint64_t key_of(double v) {
 __device__ __forceinline__ double value_of(uint64_t key) {
     return __longlong_as_double(static_cast<long long>(key >> 63 ? key & 0x7fffffffffffffffull : ~key));
 }
-__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ float value_of(uint32_t key) {
+    key += kLowestKey;
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 // Largest key of the warp; lanes that do not hold it get the same value.
 __device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(0xffffffffu, k); }
 __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
@@ -94,16 +100,46 @@ __device__ __forceinline__ float load_logit(const RouteParams& p, long long at) 
     if (p.logit_type == kLogitBf16) return as_logit(__bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]));
     return as_logit(__half2float(static_cast<const __half*>(p.logits)[at]));
 }
-// A lane's logits of a token as they stand in memory (all loads on their way together: with a look at the type at each, one load
-// waited for the other), and as numbers.
+// A lane's logits of a token, experts lane * VPL and on, as they stand in memory (all loads on their way together: with a look at
+// the type at each, one load waited for the other), and as numbers.
 template <int VPL>
 __device__ __forceinline__ void load_raw(const RouteParams& p, long long at, int lane, int experts, uint32_t (&raw)[VPL]) {
+    const int e0 = lane * VPL;
+    const bool vector = p.vector && e0 + VPL <= experts;       // (whole 16-byte pieces, or all that the lane has)
     if (p.logit_type == kLogitFp32) {
+        const uint32_t* src = static_cast<const uint32_t*>(p.logits) + at + e0;
+        if (VPL >= 4 && vector) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) raw[i] = i * 32 + lane < experts ? static_cast<const uint32_t*>(p.logits)[at + i * 32 + lane] : 0u;
+            for (int j = 0; j < VPL / 4; ++j) {
+                const uint4 v = reinterpret_cast<const uint4*>(src)[j];
+                raw[4 * j] = v.x; raw[4 * j + 1] = v.y; raw[4 * j + 2] = v.z; raw[4 * j + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) raw[i] = e0 + i < experts ? src[i] : 0u;
+        }
     } else {
+        const uint16_t* src = static_cast<const uint16_t*>(p.logits) + at + e0;
+        if (VPL >= 2 && vector) {
+            uint32_t w[VPL / 2 ? VPL / 2 : 1];
+            if constexpr (VPL >= 8) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) raw[i] = i * 32 + lane < experts ? static_cast<const uint16_t*>(p.logits)[at + i * 32 + lane] : 0u;
+                for (int j = 0; j < VPL / 8; ++j) {
+                    const uint4 v = reinterpret_cast<const uint4*>(src)[j];
+                    w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+                }
+            } else if constexpr (VPL == 4) {
+                const uint2 v = *reinterpret_cast<const uint2*>(src);
+                w[0] = v.x; w[1] = v.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t*>(src);
+            }
+#pragma unroll
+            for (int j = 0; j < VPL / 2; ++j) { raw[2 * j] = w[j] & 0xffffu; raw[2 * j + 1] = w[j] >> 16; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) raw[i] = e0 + i < experts ? src[i] : 0u;
+        }
     }
 }
 template <int VPL>
@@ -120,7 +156,7 @@ __device__ __forceinline__ void as_logits(const RouteParams& p, int lane, int ex
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane >= experts) x[i] = -INFINITY;
+        if (lane * VPL + i >= experts) x[i] = -INFINITY;
 }
 
 // Takes the key out of the warp's keys that is top_key, the one of the lowest expert where several are: that expert.  (Each key is compared
@@ -130,15 +166,15 @@ __device__ __forceinline__ uint32_t take(Key (&key)[VPL], Key top_key, int lane)
     uint32_t mine = 0xffffffffu;
 #pragma unroll
     for (int i = VPL - 1; i >= 0; --i)
-        if (key[i] == top_key) mine = i * 32 + lane;
+        if (key[i] == top_key) mine = lane * VPL + i;
     const uint32_t e = __reduce_min_sync(0xffffffffu, mine);
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-        if (e == static_cast<uint32_t>(i * 32 + lane)) key[i] = 0;
+        if (e == static_cast<uint32_t>(lane * VPL + i)) key[i] = 0;
     return e;
 }
 
-// The choice of one token by one warp: lane holds experts lane, lane + 32, ...
+// The choice of one token by one warp: lane holds experts lane * VPL, lane * VPL + 1, ...
 //
 // Keys.  Where the order of the logits is the order of the choice (no bias, and groups judged by their best) the keys
 // are those of the logits, and exact.  Otherwise two scores may be nearer to each other than 32 bits show, and which
@@ -176,7 +212,7 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const PlanParam
     }
 #pragma unroll 1
     for (int i = 0; i < VPL; ++i) {
-        const int e = i * 32 + lane;
+        const int e = lane * VPL + i;
         double c = x[i];
         if (!BY_LOGIT && x[i] != -INFINITY)
             c = (p.scoring == kScoreSoftmax ? exp(static_cast<double>(x[i]) - top) / total : 1.0 / (1.0 + exp(-static_cast<double>(x[i])))) +
@@ -187,7 +223,7 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const PlanParam
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-            if (i * 32 + lane < q.experts) keys[i * 32 + lane] = key[i];
+            if (lane * VPL + i < q.experts) keys[lane * VPL + i] = key[i];
         __syncwarp();
         const int per = q.experts / p.groups;
         uint64_t mine = 0;
@@ -210,7 +246,7 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const PlanParam
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int e = i * 32 + lane;
+            const int e = lane * VPL + i;
             if (e < q.experts && !(kept >> (e / per) & 1u)) key[i] = 0;
         }
         __syncwarp();
@@ -243,11 +279,11 @@ __device__ __forceinline__ int rank_of(uint32_t mine, int place, const uint32_t*
     return rank;
 }
 
-// x: the token's logits.  keys: shared memory of this warp (p.key_words, 16-byte aligned).  A lane whose slot is not negative has the
+// x: the token's logits.  most: above every |choice|.  keys: shared memory of this warp (p.key_words, 16-byte aligned).  A lane whose slot is not negative has the
 // expert of that slot; slots that no lane has are nobody's.  Returns how many there are.
 template <bool BY_LOGIT, int VPL>
 __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q, long long token, int lane, const float (&x)[VPL], const float (&bias)[VPL],
-                                      uint32_t* keys, int& slot, int& expert, float& weight) {
+                                      float most, uint32_t* keys, int& slot, int& expert, float& weight) {
     uint32_t key[VPL];
     float top = 0.f, total = 1.f;    // softmax: the largest logit, sum of exp(x - top)
     [[maybe_unused]] float t[VPL];   // scores
@@ -283,40 +319,49 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
     float apart = 0.f;    // decisions are sure where the values are further apart than this
     if constexpr (BY_LOGIT) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) key[i] = x[i] == -INFINITY ? 0u : key_of(x[i]);
+        for (int i = 0; i < VPL; ++i) key[i] = key_of(x[i]);
     } else {
         // Errors of a score s, in units of 2^-24 of the largest: four for the exponential, one for its argument (times s, at most
         // 0.37), five for the quotient, VPL + 5 for the softmax's total; then one of the choice.  Two compared values of two scores
         // each: four times that.
-        uint32_t most = 0u;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const float c = t[i] + bias[i];
-            const bool available = x[i] != -INFINITY && c == c && c != -INFINITY;          // (a bias of -inf or NaN masks its expert too)
-            key[i] = available ? key_of(c) : 0u;
-            most = max(most, available ? __float_as_uint(fabsf(c)) : 0u);
+            // (an expert whose logit or bias is -inf or NaN: -inf)
+            const float c = fmaxf(x[i] == -INFINITY ? -INFINITY : t[i] + bias[i], -INFINITY);
+            key[i] = key_of(c);
         }
         const float units = p.scoring == kScoreSoftmax ? __fdividef(VPL + 16.f, total) : 10.f;      // (the largest softmax score is 1 / total)
-        apart = 4.f * 5.9604645e-8f * (units + __uint_as_float(__reduce_max_sync(0xffffffffu, most)));
+        apart = 4.f * 5.9604645e-8f * (units + most);
     }
     if (p.groups > 1) {
-        // 32 / (groups rounded up to a power of two) lanes judge a group; rows of keys one word apart, against bank conflicts
-        __syncwarp();
-        const int per = q.experts / p.groups;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int e = i * 32 + lane;
-            if (e < q.experts) keys[e + (e * p.per_magic >> 20)] = key[i];
-        }
-        __syncwarp();
-        const int lanes = p.group_lanes, g = lane / lanes;
+        // A group's experts are those of direct_lanes neighbouring lanes; or, where lanes hold experts of several groups, the keys go through
+        // shared memory, 32 / (groups rounded up to a power of two) lanes judge a group, rows of keys one word apart, against
+        // bank conflicts.
+        const bool direct = p.direct_lanes != 0;
+        const int lanes = direct ? p.direct_lanes : p.group_lanes, g = lane / lanes;
         uint32_t first = 0, second = 0;
-        if (g < p.groups)
-            for (int i = lane & (lanes - 1); i < per; i += lanes) {
-                const uint32_t k = keys[g * (per + 1) + i];
-                second = max(second, min(first, k));
-                first = max(first, k);
+        if (direct) {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                second = max(second, min(first, key[i]));
+                first = max(first, key[i]);
             }
+        } else {
+            __syncwarp();
+            const int per = q.experts / p.groups;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const int e = lane * VPL + i;
+                if (e < q.experts) keys[e + (e * p.per_magic >> 20)] = key[i];
+            }
+            __syncwarp();
+            if (g < p.groups)
+                for (int i = lane & (lanes - 1); i < per; i += lanes) {
+                    const uint32_t k = keys[g * (per + 1) + i];
+                    second = max(second, min(first, k));
+                    first = max(first, k);
+                }
+        }
         for (int s = 1; s < lanes; s <<= 1) {
             const uint32_t f = __shfl_xor_sync(0xffffffffu, first, s), u = __shfl_xor_sync(0xffffffffu, second, s);
             second = max(min(first, f), max(second, u));
@@ -332,18 +377,23 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             rank += other > mine || (other == mine && h < g);
         }
         const bool keep = g < p.groups && rank < p.top_groups;
-        const uint32_t heads = __ballot_sync(0xffffffffu, keep && (lane & (lanes - 1)) == 0);      // bit h * lanes: group h is kept
         if constexpr (!BY_LOGIT) {
             const uint32_t worst = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu);
             const uint32_t best = __reduce_max_sync(0xffffffffu, keep || g >= p.groups ? 0u : mine);
             if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > apart)) apart = INFINITY;
         }
+        if (direct) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const int e = i * 32 + lane;
-            if (e < q.experts && !(heads >> ((e * p.per_magic >> 20) * lanes) & 1u)) key[i] = 0;
+            for (int i = 0; i < VPL; ++i) key[i] = keep ? key[i] : 0u;
+        } else {
+            const uint32_t heads = __ballot_sync(0xffffffffu, keep && (lane & (lanes - 1)) == 0);      // bit h * lanes: group h is kept
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const int e = lane * VPL + i;
+                if (e < q.experts && !(heads >> ((e * p.per_magic >> 20) * lanes) & 1u)) key[i] = 0;
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
     // candidates, one to a lane: cand holds their keys, ids their experts
     uint32_t* const cand = keys;
@@ -378,13 +428,19 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         __syncwarp();
         cand[lane] = 0u;
         __syncwarp();
+        int pos = 0;        // candidates of the lanes ahead: side by side in the order of the experts
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const uint32_t b = __ballot_sync(0xffffffffu, key[i] >= floor_key);
-            const int pos = n + __popc(b & ((1u << lane) - 1u));
-            if (key[i] >= floor_key && pos < 32) { cand[pos] = key[i]; ids[pos] = i * 32 + lane; }
+            pos += __popc(b & ((1u << lane) - 1u));
             n += __popc(b);
         }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (key[i] >= floor_key) {
+                if (pos < 32) { cand[pos] = key[i]; ids[pos] = lane * VPL + i; }
+                ++pos;
+            }
         __syncwarp();
         if (lane < n) { mine = cand[lane]; expert = ids[lane]; }
         rank = rank_of(mine, lane, cand, min(n, 32));
@@ -662,14 +718,21 @@ __global__ void __launch_bounds__(route_threads(VPL)) route_kernel(const RoutePa
     uint32_t ahead[VPL];     // the logits of a token are asked for while the one before is worked on
     if (warp < tokens) load_raw<VPL>(p, (first + warp) * p.logits_row_stride, lane, q.experts, ahead);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) bias[i] = !BY_LOGIT && p.bias && i * 32 + lane < q.experts ? p.bias[i * 32 + lane] : 0.f;
+    for (int i = 0; i < VPL; ++i) bias[i] = !BY_LOGIT && p.bias && lane * VPL + i < q.experts ? p.bias[lane * VPL + i] : 0.f;
+    float most = 0.f;        // above every choice: scores are at most 1
+    if constexpr (!BY_LOGIT) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (bias[i] == bias[i] && bias[i] != -INFINITY) most = fmaxf(most, fabsf(bias[i]));
+        most = 1.f + __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+    }
     for (int t = warp; t < tokens; t += warps) {
         float x[VPL];
         as_logits<VPL>(p, lane, q.experts, ahead, x);
         if (t + warps < tokens) load_raw<VPL>(p, (first + t + warps) * p.logits_row_stride, lane, q.experts, ahead);
         int slot, expert;
         float weight;
-        const int n = choose<BY_LOGIT, VPL>(p, q, first + t, lane, x, bias, keys, slot, expert, weight);
+        const int n = choose<BY_LOGIT, VPL>(p, q, first + t, lane, x, bias, most, keys, slot, expert, weight);
         const long long at = (first + t) * q.top_k;
         if (slot >= 0) {
             q.expert[at + slot] = expert;
