@@ -60,9 +60,9 @@ PlanParams plan_params(const nvfp4_routing* r, const PlanSizes& s) {
     q.tile_tokens = s.tile_tokens; q.tile_sf_rows = s.tile_sf_rows;
     q.tile_shift = s.tile_tokens == kTileFew ? 5 : 8;
     q.chunk_tokens = s.chunk_tokens; q.chunks = s.chunks;
-    // all pairs of a chunk at once where 28 KB of bits allow it
+    // all pairs of a chunk at once where 36 KB of bits allow it
     const int in_chunk = r->tokens < s.chunk_tokens ? r->tokens : s.chunk_tokens;
-    const long long needed = (static_cast<long long>(in_chunk) * r->top_k + 31) / 32, most = 7168 / r->experts;
+    const long long needed = (static_cast<long long>(in_chunk) * r->top_k + 31) / 32, most = 9216 / r->experts;
     q.bit_words = static_cast<int>(needed < most ? needed : most);
     q.expert = r->expert; q.row = r->row; q.offset = r->offset;
     int* words = static_cast<int*>(r->plan);
