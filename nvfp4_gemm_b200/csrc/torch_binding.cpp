@@ -10,8 +10,8 @@
 // 3.75 us a pass; a first call on new tensors 28.5 -> 17.6 us, waited for).
 #include <Python.h>
 
-#include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -276,17 +276,16 @@ void rows_of(const at::Tensor& t, const char* name) {
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// What a call makes itself, on the device of `on`.
-at::Tensor fresh(const at::Tensor& on, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, on.options().dtype(type)); }
-
-// Several results in one allocation (each costs the caching allocator more than a small kernel's launch leaves room for): tensors
-// of their own on one storage, which lives as long as any of them.
+// Results of a call: tensors of their own on one allocation from torch's allocator (current device and stream), which lives as long
+// as any of them.  Straight from the allocator: an at::empty() for each took longer than a small kernel runs.
 class Slab {
 public:
-    Slab(const at::Tensor& on, int64_t bytes) : base_(at::empty({bytes}, on.options().dtype(at::kByte).requires_grad(false))) {}
+    explicit Slab(int64_t bytes)
+        : storage_(c10::Storage::use_byte_size_t(), static_cast<size_t>(bytes), c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes)),
+                   c10::cuda::CUDACachingAllocator::get(), false) {}
     static int64_t room(int64_t bytes) { return (bytes + 255) & ~int64_t{255}; }
     at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
-        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(), c10::scalarTypeToTypeMeta(type));
+        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(storage_), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
         const int64_t item = static_cast<int64_t>(c10::elementSize(type));
         impl->set_storage_offset(used_ / item);
         impl->set_sizes_contiguous(sizes);
@@ -295,9 +294,13 @@ public:
     }
 
 private:
-    at::Tensor base_;
+    c10::Storage storage_;
     int64_t used_ = 0;
 };
+// (with the tensors' device current)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+    return Slab(c10::multiply_integers(sizes) * static_cast<int64_t>(c10::elementSize(type))).take(sizes, type);
+}
 
 PyObject* status_object(int rc) { return PyLong_FromLong(rc); }
 
@@ -324,12 +327,12 @@ struct Routing {
     int status;
     at::Tensor expert, weight;
     // new rows, offsets and plan for [tokens, top_k] choices, and the choices and their weights too (choose)
-    Routing(const at::Tensor& on, int64_t tokens, int64_t top_k, int64_t experts, bool choose) {
+    Routing(int64_t tokens, int64_t top_k, int64_t experts, bool choose) {
         int64_t plan_bytes = 0;
         status = size(tokens, top_k, experts, &plan_bytes);
         if (status) return;
         const int64_t per_pair = Slab::room(tokens * top_k * 4);
-        Slab slab(on, per_pair * (choose ? 3 : 1) + Slab::room((experts + 1) * 4) + Slab::room(plan_bytes));
+        Slab slab(per_pair * (choose ? 3 : 1) + Slab::room((experts + 1) * 4) + Slab::room(plan_bytes));
         row = slab.take({tokens, top_k}, at::kInt);
         offset = slab.take({experts + 1}, at::kInt);
         plan = slab.take({plan_bytes / 4}, at::kInt);
@@ -403,7 +406,7 @@ PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         o.renormalize = int_arg(args[7]);
         o.scale = static_cast<float>(float_arg(args[8]));
         const c10::cuda::CUDAGuard guard(logits.device());
-        Routing routing(logits, logits.size(0), top_k, logits.size(1), true);
+        Routing routing(logits.size(0), top_k, logits.size(1), true);
         if (routing.status) return status_object(routing.status);
         o.logits = logits.data_ptr();
         o.logits_row_stride = row_stride(logits);
@@ -422,7 +425,7 @@ PyObject* py_plan(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         if (experts.dim() != 2 || experts.scalar_type() != at::kInt || !experts.is_contiguous())
             raise(PyExc_ValueError, "experts must be a contiguous int32 tensor [tokens, top_k]");
         const c10::cuda::CUDAGuard guard(experts.device());
-        Routing routing(experts, experts.size(0), experts.size(1), int_arg(args[1]), false);
+        Routing routing(experts.size(0), experts.size(1), int_arg(args[1]), false);
         if (routing.status) return status_object(routing.status);
         routing.r.expert = experts.data_ptr<int32_t>();
         const int rc = on_current_stream(experts, [&](void* stream) { return nvfp4_plan_experts(&routing.r, stream); });
@@ -444,7 +447,7 @@ PyObject* py_quantize_routed(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         if (routing.r.tokens != x.size(0)) raise(PyExc_ValueError, "x must have a row per token of the routing");
         const int64_t k = size_arg(x.size(1), "the width of x");
         const int64_t rows = routing.row.numel();
-        Slab slab(x, Slab::room(rows * (k / 2)) + Slab::room(routing.sf_rows * (k / 16)));
+        Slab slab(Slab::room(rows * (k / 2)) + Slab::room(routing.sf_rows * (k / 16)));
         const at::Tensor packed = slab.take({rows, k / 2}, at::kFloat4_e2m1fn_x2), sf = slab.take({routing.sf_rows * (k / 16)}, at::kFloat8_e4m3fn);
         const void* const src = x.data_ptr();
         void *const codes = packed.data_ptr(), *const scales = sf.data_ptr();
@@ -515,7 +518,7 @@ PyObject* py_expert_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         at::Tensor out, out_sf;
         if (to_nvfp4) {
             if (args[12] != Py_None) raise(PyExc_ValueError, "out is for the fp16 result");
-            Slab slab(a, Slab::room(rows * (n_out / 2)) + Slab::room(routing.sf_rows * (n_out / 16)));
+            Slab slab(Slab::room(rows * (n_out / 2)) + Slab::room(routing.sf_rows * (n_out / 16)));
             out = slab.take({rows, n_out / 2}, at::kFloat4_e2m1fn_x2);
             out_sf = slab.take({routing.sf_rows * (n_out / 16)}, at::kFloat8_e4m3fn);
             p.output = NVFP4_OUT_NVFP4;
@@ -528,7 +531,7 @@ PyObject* py_expert_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             out = *t;
             p.out_row_stride = row_stride(out);
         } else {
-            out = fresh(a, {rows, n_out}, at::kHalf);
+            out = fresh({rows, n_out}, at::kHalf);
             p.out_row_stride = n_out;
         }
         p.out = out.data_ptr();
@@ -563,7 +566,7 @@ PyObject* py_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                 if (t->size(0) != tokens || t->size(1) != n || t->scalar_type() != type) raise_value("%s must be [tokens, n] of the output's type", names[i]);
             }
         const c10::cuda::CUDAGuard guard(y.device());
-        const at::Tensor out = given ? *given : fresh(y, {tokens, n}, type);
+        const at::Tensor out = given ? *given : fresh({tokens, n}, type);
         const int32_t y_rows = size_arg(y.size(0), "y"), t = size_arg(tokens, "the number of tokens"), top_k = size_arg(rows.size(1), "top_k"), cols = size_arg(n, "n");
         const void *const src = y.data_ptr(), *const add = residual ? residual->data_ptr() : nullptr;
         const int32_t* const row = rows.data_ptr<int32_t>();
