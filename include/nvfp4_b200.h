@@ -298,7 +298,8 @@ int nvfp4_gemm_static_scratch(const nvfp4_problem* problem, int workers, void* s
  *
  * nvfp4_routing is the result of the router on the device; all its memory is the caller's, and none of these
  * functions keeps anything of a call.  Sizes come from nvfp4_routing_plan().  Not more than 1024 experts, 32 choices and
- * 2^31 - 1 pairs; tokens may be 0.
+ * 2^31 - 1 pairs; tokens may be 0.  Make the first call on a device outside any graph capture; calls may overlap on
+ * streams, and be captured and replayed, as their memory allows.
  */
 typedef struct nvfp4_routing {
     int32_t tokens, top_k, experts;

@@ -444,3 +444,57 @@ def test_scores_at_the_border_of_what_32_bits_tell_apart(ex):
             exp, _ = ref.route(logits[t:t + 1], top_k, scoring=scoring, bias=b32)
             r = ex.route(logits[t:t + 1].cuda(), top_k, scoring=scoring, bias=b32.cuda())
             assert r.experts.cpu().tolist() == exp.tolist(), (scoring, t)
+
+
+def test_infinite_biases_and_padded_tokens_by_scores(ex, lib):
+    """A bias of +inf takes its expert always; tokens without any expert stand among others, in the paths that compare scores."""
+    g = _gen(12)
+    for experts, top_k in ((64, 4), (256, 8)):
+        x = torch.randn((70, experts), generator=g)
+        x[::7] = -INF
+        x[3, 1:] = -INF
+        bias = torch.randn(experts, generator=g) * 0.1
+        for b in (bias, torch.where(torch.arange(experts) % 31 == 5, torch.tensor(INF), bias)):
+            for kw in (dict(scoring="sigmoid"), dict(), dict(scoring="sigmoid", groups=8, top_groups=3, group_score="top2")):
+                r = ex.route(x.cuda(), top_k, bias=b.cuda(), **kw)
+                _check_routing(lib, r, x, top_k, experts, bias=b, **kw)
+
+
+def test_one_expert_takes_every_row(ex, lib):
+    for tokens in (3, 300):
+        r, rows, a = _rows(ex, lib, tokens, 1, 1, 256, tokens)
+        w, w_sf, wv = _weights(1, 256, 256, 2)
+        y = ex.expert_gemm(rows, r, w, w_sf)
+        z, size = ref.expert_product(a, r.offsets.cpu(), wv, None, None)
+        _check_product(y[:int(r.offsets[-1])], z, size, "none", 1.0, 256)
+
+
+def test_gpu_side_refusals(ex, lib):
+    from nvfp4_gemm_b200 import _lib
+    r = ex.route(torch.randn((6, 16), device="cuda"), 2)
+    rows = ex.quantize_routed(torch.randn((6, 256), device="cuda").half(), r)
+    w, w_sf, _ = _weights(16, 128, 256, 1)
+    with pytest.raises(ValueError, match="row per token"):
+        ex.quantize_routed(torch.randn((5, 256), device="cuda").half(), r)
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        ex.quantize_routed(torch.randn((6, 256), device="cuda"), r)
+    with pytest.raises(ValueError, match="plan does not belong"):
+        ex.expert_gemm(rows, r._replace(num_experts=700), w, w_sf)
+    with pytest.raises(ValueError, match="disagree"):
+        ex.expert_gemm(rows, r, w[:, :64], w_sf)
+    with pytest.raises(ValueError, match="512-byte atoms"):
+        ex.expert_gemm(rows, r, w, w_sf[..., :8])
+    with pytest.raises(ValueError, match="routed operand"):
+        ex.expert_gemm((rows.packed, rows.sf[:-16]), r, w, w_sf)
+    with pytest.raises(ValueError, match="alpha"):
+        ex.expert_gemm(rows, r, w, w_sf, alpha=torch.ones(15, device="cuda"))
+    with pytest.raises(ValueError, match="bias"):
+        ex.expert_gemm(rows, r, w, w_sf, bias=torch.ones((16, 128), device="cuda"))
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ex.combine(torch.zeros((12, 128), dtype=torch.float16, device="cuda"), r.rows.cpu(), r.weights)
+    with pytest.raises(_lib.Nvfp4Error, match="top_k = 17 of 16"):
+        ex.route(torch.randn((6, 16), device="cuda"), 17)
+    with pytest.raises(_lib.Nvfp4Error, match="groups"):
+        ex.route(torch.randn((6, 16), device="cuda"), 2, groups=5)
+    with pytest.raises(ValueError, match="output's type"):
+        ex.combine(torch.zeros((12, 128), dtype=torch.float16, device="cuda"), r.rows, r.weights, residual=torch.zeros((6, 128), device="cuda"), dtype=torch.float16)
