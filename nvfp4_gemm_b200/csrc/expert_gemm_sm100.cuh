@@ -18,6 +18,12 @@
 // where a thread has columns t and t + 8 of the output for the same row: gate and up, alternating in groups of eight,
 // meet in a thread.  The finished fp16 pairs are turned round by stmatrix on their way to shared memory and leave as 16-byte pieces.
 //
+// Bounds and figures (us; weights E x n x k, rows in all).  Few rows: HBM, each touched expert's weights once: 8 x 4096 x 7168 for one token
+// 20.7 (6.4 TB/s), 32 x 4096 x 4096 for 64 tokens x 4 45.4, 32 x 7168 x 2048 for 64 x 8 39.8 (6.6 TB/s).  Many rows: what the dense pair kernel
+// is bound by, and its rates: 65536 rows evenly over 32 experts, 4096 x 7168 693-703 (5.5 PFLOP/s; dense, 8 batches 677), 7168 x 2048 426-437 (dense 434); in
+// a loop the 1000 W limit holds the SM clock at 1.15 to 1.25 GHz.  The epilogue of a 256 x 256 tile takes 2.8 of its own, 3.3 with its stores, beside
+// 3.0 of MMAs at k = 2048.
+//
 // Every wait is bounded.  No load uses cluster multicast.
 #pragma once
 #include "gemm_sm100.cuh"

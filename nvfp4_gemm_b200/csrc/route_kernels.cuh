@@ -183,6 +183,9 @@ __device__ __forceinline__ uint32_t take(Key (&key)[VPL], Key top_key, int lane)
 // apart than the bound allows, the candidates' scores are computed and ranked in 64 bits; where groups are not, the token
 // is chosen again in 64 bits (choose_exactly).
 //
+// Bound by instructions: 8192 tokens of 256 experts take 23.6 us by sigmoid, bias and eight groups, 16.1 by softmax (8.5 of either for the order of the
+// pairs behind it); one token of 64 experts 4.2, of 256 5.2.
+//
 // Ranking.  The top_k largest keys are not below the top_k-th largest of the lanes' maxima.  What is not below it, seldom much
 // more than top_k keys, is put side by side, one to a lane, and each counts those ahead of it.  (Taking the largest top_k
 // times from all lanes' keys took 919 instructions a token of 256 experts, and waited for most of them.)
@@ -768,7 +771,8 @@ struct QuantizeRoutedParams {
 
 constexpr int kRoutedCols = 512;     // columns per warp
 // A lane takes one scale block (16 elements, 32 bytes) of a token, a warp 512 columns; the codes and scales, made once, are
-// stored in each of the token's rows.
+// stored in each of the token's rows.  Bound by what it writes: 8192 x 8 rows of 7168 take 88 us (4.3 TB/s), 55 without the scales, four bytes of
+// each row and four blocks in a sector of their own, which cost L2 as many writes as the codes; 8192 x 2 x 4096 20 (5.2 TB/s); one token 2.1.
 template <bool BF16, bool kWide>
 __global__ void __launch_bounds__(256) quantize_routed_kernel(const QuantizeRoutedParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
