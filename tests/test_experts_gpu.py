@@ -498,3 +498,39 @@ def test_gpu_side_refusals(ex, lib):
         ex.route(torch.randn((6, 16), device="cuda"), 2, groups=5)
     with pytest.raises(ValueError, match="output's type"):
         ex.combine(torch.zeros((12, 128), dtype=torch.float16, device="cuda"), r.rows, r.weights, residual=torch.zeros((6, 128), device="cuda"), dtype=torch.float16)
+
+
+@pytest.mark.parametrize("tokens,kernel", [(4, "expert_gemm_t32"), (64, "expert_gemm_2cta_t256")])
+def test_a_product_that_gives_up_reports_it(ex, lib, tokens, kernel):
+    """With a limit of a nanosecond waits run out while a long product's operands are still streaming in.  The launch ends, the host hears
+    of it, and what runs next is right."""
+    from nvfp4_gemm_b200 import _lib, submission
+    from nvfp4_gemm_b200.inputs import FP4_DTYPE, SF_DTYPE
+    n, k = 256, 1 << 23
+    r = ex.plan(torch.zeros((tokens, 1), dtype=torch.int32, device="cuda"), 1)
+    w = torch.full((1, n, k // 2), 0x02, dtype=torch.uint8, device="cuda").permute(1, 2, 0).view(FP4_DTYPE)              # 1 and 0 in turn
+    w_sf = torch.full((1, n // 128, k // 64, 32, 4, 4), 0x08, dtype=torch.uint8, device="cuda").permute(3, 4, 1, 5, 2, 0).view(SF_DTYPE)   # 2^-6
+    sf_rows = ctypes.c_int64()
+    assert lib.nvfp4_routing_plan(tokens, 1, 1, None, None, ctypes.byref(sf_rows)) == 0
+    rows = ex.RoutedRows(torch.full((tokens, k // 2), 0x02, dtype=torch.uint8, device="cuda"),
+                         torch.full((sf_rows.value * (k // 16),), 0x08, dtype=torch.uint8, device="cuda"))
+    r2, small, a = _rows(ex, lib, 40, 2, 4, 512, 3)
+    w2, w2_sf, w2v = _weights(4, 256, 512, 3)
+    z, size = ref.expert_product(a, r2.offsets.cpu(), w2v, None, None)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        prev = lib.nvfp4_set_wait_timeout_ns(1)
+        try:
+            ex.expert_gemm(rows, r, w, w_sf)
+        finally:
+            lib.nvfp4_set_wait_timeout_ns(prev)
+        assert submission.last_kernel() == kernel
+        with pytest.raises(_lib.Nvfp4Error) as e:
+            submission.check_status()
+        assert e.value.code == _lib.NVFP4_ERR_DEVICE_TIMEOUT
+        y = ex.expert_gemm(small, r2, w2, w2_sf)
+        submission.check_status()
+        _check_product(y[:int(r2.offsets[-1])], z, size, "none", 1.0, 512)
+    y = ex.expert_gemm(rows, r, w, w_sf, alpha=torch.full((1,), 2.0 ** -4, device="cuda"))
+    submission.check_status()
+    assert torch.equal(y, torch.full_like(y, k // 2 * 2.0 ** -16))      # exact
