@@ -1222,7 +1222,8 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
         if (*abort_flag) {
             // Some wait ran out.  Give copies still in flight time to land in shared memory before
             // the CTA retires, then report.
-            __nanosleep(20000);
+            if constexpr (EPI_EX == kEpiResidualFp16) let_copies_land();     // (a residual's tile may be on its way too)
+            else __nanosleep(20000);
             if (threadIdx.x == 0) {
                 *reinterpret_cast<volatile int*>(p.status) = kStatusWaitTimeout;
                 __threadfence_system();

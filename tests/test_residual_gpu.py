@@ -118,3 +118,35 @@ def test_residual_refusals(sub, lib):
     shifted = torch.zeros((20, 264), dtype=torch.float16, device="cuda")[:, 4:260].unsqueeze(2)
     with pytest.raises(_lib.Nvfp4Error, match="16-byte aligned"):
         sub.gemm_epilogue(data, residual=shifted)
+
+
+def test_a_product_with_residual_that_gives_up_reports_it(sub, lib, oracle):
+    """With a limit of a nanosecond waits run out while operands, and the residual's tile, are still on their way."""
+    from nvfp4_gemm_b200 import _lib
+    from nvfp4_gemm_b200.inputs import FP4_DTYPE, SF_DTYPE
+    m, n, k = 256, 256, 1 << 22
+    codes = torch.full((1, m, k // 2), 0x02, dtype=torch.uint8, device="cuda").permute(1, 2, 0).view(FP4_DTYPE)        # 1 and 0 in turn
+    atoms = torch.full((1, 2, k // 64, 32, 4, 4), 0x08, dtype=torch.uint8, device="cuda").permute(3, 4, 1, 5, 2, 0).view(SF_DTYPE)   # 2^-6
+    c = torch.empty((1, m, n), dtype=torch.float16, device="cuda").permute(1, 2, 0)
+    data = (codes, codes, None, None, atoms, atoms, c)
+    small, bias, residual = _inputs((300, 512, 512, 1), 36)
+    exp = _expected(oracle, small, bias, "none", residual)
+    one = torch.ones_like(c)
+    kw = dict(cta_group=2, tile_n=256, grid=2, split_k=1)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        prev = lib.nvfp4_set_wait_timeout_ns(1)
+        try:
+            sub.gemm_epilogue(data, residual=one, **kw)
+        finally:
+            lib.nvfp4_set_wait_timeout_ns(prev)
+        assert sub.last_kernel() == "gemm_2cta_n256_s4_residual_tmastore"
+        with pytest.raises(_lib.Nvfp4Error) as e:
+            sub.check_status()
+        assert e.value.code == _lib.NVFP4_ERR_DEVICE_TIMEOUT
+        out = sub.gemm_epilogue(small, bias=bias, residual=residual)
+        sub.check_status()
+        assert_bit_exact(out, exp, what="after a launch that gave up")
+    sub.gemm_epilogue(data, residual=one, **kw)
+    sub.check_status()
+    assert torch.equal(c, torch.full_like(c, k // 2 * 2.0 ** -12 + 1))       # 512 + 1: exact
