@@ -965,6 +965,7 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                     for (int i = 0; i < kMyRelease; ++i) ptx::tc_ld_32cols(t_acc + my_chunk(i) * 32, held[i]);
                     ptx::tc_wait_ld();
                     release_acc();
+                    const bool plain_sum = p.bias == nullptr && p.activation == kActNone;
                     const int w_last = whole_tile ? worker : unit_owner(tile * KT + KT - 1, n_workers, p.total_units);
                     if (!whole_tile && !wait_for_others(p.counters + worker * CG + cta_rank, KT - (k1 - k0))) break;
                     auto finish = [&](int ci, const uint32_t (&lo)[32], const uint32_t (&hi)[32]) {
@@ -984,21 +985,28 @@ __global__ void __launch_bounds__(GemmSmem<CG, BN, STAGES, TMA_STORE, EPI_KB, KS
                             }
                         }
                         uint8_t* const buf = staging_gen + ci * 4096 + lane * 128;     // this thread's row, 16-byte pieces, 128-byte swizzle
+                        auto piece = [&](int j) { return reinterpret_cast<uint4*>(buf + ((j ^ (lane & 7)) << 4)); };
+                        uint4 res[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) res[j] = *piece(j);
+                        if (!plain_sum) {        // (a branch around the loop: in it, it would keep the 16 columns of a turn apart)
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                if (p.bias) {
+                                    const uint4* b = reinterpret_cast<const uint4*>(smem_gen + S::kBiasOff + (warp - 2) * S::kBiasPerWarp + ci * 128 + h * 32);
+                                    const uint4 now[2] = {b[0], b[1]};
+                                    add_fp16x16(now, &s[16 * h]);
+                                }
+                                activate16(p.activation, &s[16 * h]);
+                            }
+                        }
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
-                            if (p.bias) {
-                                const uint4* b = reinterpret_cast<const uint4*>(smem_gen + S::kBiasOff + (warp - 2) * S::kBiasPerWarp + ci * 128 + h * 32);
-                                const uint4 now[2] = {b[0], b[1]};
-                                add_fp16x16(now, &s[16 * h]);
-                            }
-                            activate16(p.activation, &s[16 * h]);
-                            uint4* const at0 = reinterpret_cast<uint4*>(buf + (((2 * h) ^ (lane & 7)) << 4));
-                            uint4* const at1 = reinterpret_cast<uint4*>(buf + (((2 * h + 1) ^ (lane & 7)) << 4));
-                            const uint4 res[2] = {*at0, *at1};
-                            add_fp16x16(res, &s[16 * h]);
-                            *at0 = pack8_fp16(&s[16 * h]);
-                            *at1 = pack8_fp16(&s[16 * h + 8]);
+                            const uint4 now[2] = {res[2 * h], res[2 * h + 1]};
+                            add_fp16x16(now, &s[16 * h]);
                         }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) *piece(j) = pack8_fp16(&s[8 * j]);
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0 && mb * kBM + quad * 32 < p.M) {
