@@ -426,6 +426,25 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             ahead += (o.x > best) + (o.y > best) + (o.z > best) + (o.w > best);
         }
         uint32_t floor_key = least > 32 ? 0u : __reduce_min_sync(0xffffffffu, ahead < least ? best : 0xffffffffu);
+        if (floor_key == 0) {
+            // Fewer lanes than that have anything (few groups or experts are left, a lane's experts are neighbours): the least-th largest
+            // key itself, from one value to the next.
+            // (8192 tokens, two of eight groups of 256 experts: 29 us; all of them a candidate, more than lanes, and chosen in 64 bits: 56)
+            int keys_left = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) keys_left += __popc(__ballot_sync(0xffffffffu, key[i] != 0));
+            uint32_t above = 0xffffffffu;
+            for (int left = keys_left > 32 ? least : 0; left > 0;) {
+                uint32_t next = 0u;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) next = max(next, key[i] < above ? key[i] : 0u);
+                next = warp_max(next);
+                if (next == 0) break;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) left -= __popc(__ballot_sync(0xffffffffu, key[i] == next));
+                floor_key = above = next;
+            }
+        }
         if (!BY_LOGIT && floor_key) floor_key = key_of(value_of(floor_key) - apart);
         floor_key = max(floor_key, 1u);
         __syncwarp();
