@@ -534,3 +534,21 @@ def test_a_product_that_gives_up_reports_it(ex, lib, tokens, kernel):
     y = ex.expert_gemm(rows, r, w, w_sf, alpha=torch.full((1,), 2.0 ** -4, device="cuda"))
     submission.check_status()
     assert torch.equal(y, torch.full_like(y, k // 2 * 2.0 ** -16))      # exact
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top_k", [(256, 8, 1, 8), (256, 8, 2, 8), (384, 8, 2, 8), (512, 8, 1, 8), (512, 32, 3, 32), (64, 16, 2, 7), (1024, 4, 1, 32)])
+@pytest.mark.parametrize("kw", [dict(), dict(scoring="sigmoid", bias=True), dict(bias=True, group_score="top2")], ids=str)
+def test_choices_from_few_groups(ex, lib, experts, groups, top_groups, top_k, kw):
+    """What is left are the experts of a few lanes: fewer lanes than choices, and up to many more experts than lanes."""
+    g = _gen(experts + top_k)
+    x = torch.randn((40, experts), generator=g)
+    x[5, ::2] = -INF
+    x[6] = -INF
+    x[6, 3] = 0.0
+    kw = dict(kw, groups=groups, top_groups=top_groups)
+    if kw.get("bias"):
+        kw["bias"] = torch.randn(experts, generator=g) * 0.2
+    if top_groups * (experts // groups) < top_k:
+        pytest.skip("fewer experts in the groups than choices")
+    r = ex.route(x.cuda(), top_k, **{**kw, **({"bias": kw["bias"].cuda()} if "bias" in kw else {})})
+    _check_routing(lib, r, x, top_k, experts, **kw)
