@@ -110,8 +110,10 @@ int empty_plan(const PlanParams& q, cudaStream_t stream) {
     return NVFP4_OK;
 }
 
+constexpr size_t kPlaceSmem = 116 * 1024;
+constexpr int kPlaceMostCtas = 120;
 size_t plan_smem(const PlanParams& q) {
-    const int per_expert = (q.bit_words | 1) < 2 ? 2 : (q.bit_words | 1);     // (the place kernel keeps two sums there)
+    const int per_expert = (q.bit_words | 1) < 3 ? 3 : (q.bit_words | 1);     // (the place kernel keeps three sums there)
     return (plan_head_words(q.experts) + static_cast<size_t>(q.experts) * per_expert) * sizeof(int);
 }
 
@@ -124,10 +126,16 @@ int allow_smem(DeviceCtx* c, int variant, const void* kernel, size_t bytes) {
     return NVFP4_OK;
 }
 
+template <int CHUNKS>
+int place(DeviceCtx* c, int variant, const PlanParams& q, cudaStream_t stream, const char* name) {
+    constexpr int kChunks = kPlaceCluster * CHUNKS;
+    const size_t smem = plan_smem(q) > kPlaceSmem ? plan_smem(q) : kPlaceSmem;
+    if (int rc = allow_smem(c, variant, reinterpret_cast<const void*>(place_kernel<CHUNKS>), smem)) return rc;
+    return launch(place_kernel<CHUNKS>, (q.chunks + kChunks - 1) / kChunks * kPlaceCluster, kPlaceThreads, smem, kPlaceCluster, stream, name, q);
+}
 int place(DeviceCtx* c, const PlanParams& q, cudaStream_t stream, const char* name) {
     if (q.chunks <= 1) return NVFP4_OK;
-    if (int rc = allow_smem(c, 74, reinterpret_cast<const void*>(place_kernel), plan_smem(q))) return rc;
-    return launch(place_kernel, (q.chunks + kPlaceCluster - 1) / kPlaceCluster * kPlaceCluster, kPlaceThreads, plan_smem(q), kPlaceCluster, stream, name, q);
+    return q.chunks > kPlaceMostCtas ? place<2>(c, 74, q, stream, name) : place<1>(c, 88, q, stream, name);
 }
 
 template <bool BY_LOGIT, int VPL>
@@ -265,8 +273,9 @@ int nvfp4_plan_experts(const nvfp4_routing* r, void* stream_v) {
     if (int rc = check_device(&c)) return rc;
     const PlanParams q = plan_params(r, s);
     if (r->tokens == 0) return empty_plan(q, stream);
-    if (int rc = allow_smem(c, 75, reinterpret_cast<const void*>(plan_kernel), plan_smem(q))) return rc;
-    if (int rc = launch(plan_kernel, q.chunks, kPlaceThreads, plan_smem(q), 1, stream, "plan_experts", q)) return rc;
+    const size_t smem = q.chunks > 1 && plan_smem(q) < kPlaceSmem ? kPlaceSmem : plan_smem(q);
+    if (int rc = allow_smem(c, 75, reinterpret_cast<const void*>(plan_kernel), smem)) return rc;
+    if (int rc = launch(plan_kernel, q.chunks, kPlaceThreads, smem, 1, stream, "plan_experts", q)) return rc;
     return place(c, q, stream, "plan_experts_place");
 }
 

@@ -558,43 +558,11 @@ __device__ __forceinline__ void scan_experts(const int* count, int* row0, int* t
     __syncthreads();
 }
 
-// Rows of a chunk's pairs.  next[e]: how many pairs of expert e stand before the chunk (changed here); bits: experts x (bit_words | 1) words.
-// Pairs are ranked 32 * words at a time by a bit per pair and expert, so that the order is that of the pairs whichever
-// thread comes first, and the same expert twice in a token gets two rows.
-__device__ __forceinline__ void place_pairs(const PlanParams& q, long long first_pair, int pairs, const int* row0, const int* tile0, int* next,
-                                            uint32_t* bits) {
-    const int words = q.bit_words, batch = 32 * words, stride = words | 1;     // (odd: an expert's words and the next one's in other banks)
-    for (int base = 0; base < pairs; base += batch) {
-        const int here = min(batch, pairs - base), used = (here + 31) >> 5;
-        for (int i = threadIdx.x; i < q.experts * stride; i += blockDim.x) bits[i] = 0u;
-        __syncthreads();
-        for (int i = threadIdx.x; i < here; i += blockDim.x) {
-            const int e = q.expert[first_pair + base + i];
-            if (e >= 0 && e < q.experts) atomicOr(&bits[e * stride + (i >> 5)], 1u << (i & 31));
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < here; i += blockDim.x) {
-            const int e = q.expert[first_pair + base + i];
-            int row = -1, sf_row = -1;
-            if (e >= 0 && e < q.experts) {
-                int rank = next[e] + __popc(bits[e * stride + (i >> 5)] & ((1u << (i & 31)) - 1u));
-#pragma unroll 4
-                for (int w = 0; w < (i >> 5); ++w) rank += __popc(bits[e * stride + w]);
-                row = row0[e] + rank;
-                sf_row = (tile0[e] + (rank >> q.tile_shift)) * q.tile_sf_rows + (rank & (q.tile_tokens - 1));
-            }
-            q.row[first_pair + base + i] = row;
-            q.sf_row[first_pair + base + i] = sf_row;
-        }
-        if (base + batch >= pairs) break;
-        __syncthreads();
-        for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
-            int n = 0;
-            for (int w = 0; w < used; ++w) n += __popc(bits[e * stride + w]);
-            next[e] += n;
-        }
-        __syncthreads();
-    }
+// A pair's row and the row of its scales, where its rank among the expert's pairs is known.
+__device__ __forceinline__ void put_rows(const PlanParams& q, long long pair, int e, int rank, const int* row0, const int* tile0) {
+    const bool some = e >= 0 && e < q.experts;
+    q.row[pair] = some ? row0[e] + rank : -1;
+    q.sf_row[pair] = some ? (tile0[e] + (rank >> q.tile_shift)) * q.tile_sf_rows + (rank & (q.tile_tokens - 1)) : -1;
 }
 
 // offsets and the tile table, by the threads of one CTA (all of them look at row0 / tile0 of shared memory)
@@ -616,21 +584,38 @@ struct PlanSmem {
           bits(reinterpret_cast<uint32_t*>(smem + plan_head_words(experts))) {}
 };
 
-// One chunk's share of the order, where the counts of all chunks are known (16 bits each).  The eight CTAs of a cluster share the work of
-// adding them up: each sums every eighth chunk, over all chunks and over those ahead of the cluster's, and takes the others' sums from their
-// shared memory.  (Each CTA for itself: 148 CTAs read the same 75 KB of 256 experts' counts in 8000 cycles.)
+// One or two chunks' share of the order, where the counts of all chunks (16 bits each) and every pair's rank in its chunk are known.  The eight CTAs of a
+// cluster share the work of adding the counts up: each sums every eighth chunk, over all chunks and over those ahead of the cluster's, and takes the
+// others' sums from their shared memory.  (Each CTA for itself: 148 CTAs read the same 75 KB of 256 experts' counts in 8000 cycles.)
+// Two chunks where one each would be more CTAs than clusters of eight find room for at one CTA an SM (TWO_US).
 constexpr int kPlaceCluster = 8;
-__global__ void __launch_bounds__(kPlaceThreads) place_kernel(const PlanParams q) {
+template <int CHUNKS>
+__global__ void __launch_bounds__(kPlaceThreads, 1) place_kernel(const PlanParams q) {
+    constexpr int kAtOnce = 2 * CHUNKS;
     extern __shared__ __align__(16) int plan_smem[];
     const PlanSmem s(plan_smem, q.experts);
     int* const sums = reinterpret_cast<int*>(s.bits);       // [2][experts]: ahead of the cluster's chunks, of all (this CTA's share)
-    ptx::grid_dependency_launch_dependents();
+    int* const next1 = sums + 2 * q.experts;                // s.next of the second chunk
     ptx::grid_dependency_wait();
-    const int chunk = blockIdx.x, lane = threadIdx.x & 31;
-    const int rank = static_cast<int>(ptx::cluster_ctarank()), cluster_first = chunk - rank;
+    const int lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(ptx::cluster_ctarank());
+    const int cluster_first = (static_cast<int>(blockIdx.x) - rank) * CHUNKS, chunk = static_cast<int>(blockIdx.x) * CHUNKS;
     const int count_row = counts_row(q.experts);
+    const int chunk_pairs = q.chunk_tokens * q.top_k;
+    const long long first = static_cast<long long>(chunk) * chunk_pairs;
+    const int pairs = static_cast<int>(max(min(static_cast<long long>(CHUNKS) * chunk_pairs, static_cast<long long>(q.tokens) * q.top_k - first), 0ll));
+    // this thread's first pairs: asked for ahead of everything that it waits for
+    int e[kAtOnce], r[kAtOnce];
+    auto ask = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int i = base + j * kPlaceThreads + threadIdx.x;
+            if (i < pairs) { e[j] = q.expert[first + i]; r[j] = q.row[first + i]; }
+        }
+    };
+    ask(0);
     // a warp takes sixteen experts (a sector of a chunk's row), a lane a chunk
-    for (int e0 = (threadIdx.x >> 5) * 16; e0 < q.experts; e0 += (blockDim.x >> 5) * 16) {
+    for (int e0 = (threadIdx.x >> 5) * 16; e0 < q.experts; e0 += kPlaceThreads / 32 * 16) {
         int before[16] = {}, all[16] = {};
         for (int c = rank + kPlaceCluster * lane; c < q.chunks; c += kPlaceCluster * 32) {
             const uint4* src = reinterpret_cast<const uint4*>(q.counts + static_cast<long long>(c) * count_row + e0);
@@ -650,59 +635,111 @@ __global__ void __launch_bounds__(kPlaceThreads) place_kernel(const PlanParams q
         }
     }
     ptx::cluster_arrive();
-    // the chunks of this cluster ahead of this one
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
-        int n = 0;
+    // the chunks of this cluster ahead of this CTA's (last)
+    for (int x = threadIdx.x; x < q.experts; x += kPlaceThreads) {
+        int n = 0, own = 0;
 #pragma unroll
-        for (int i = 0; i < kPlaceCluster - 1; ++i)
-            if (i < rank && cluster_first + i < q.chunks) n += q.counts[static_cast<long long>(cluster_first + i) * count_row + e];
-        s.next[e] = n;
+        for (int i = 0; i < kPlaceCluster * CHUNKS - 1; ++i) {
+            const int c = cluster_first + i;
+            const int here = c <= (CHUNKS > 1 ? chunk : chunk - 1) && c < q.chunks ? q.counts[static_cast<long long>(c) * count_row + x] : 0;
+            if (c == chunk) own = here;
+            else n += here;
+        }
+        s.next[x] = n;
+        if (CHUNKS > 1) next1[x] = n + own;
     }
     ptx::cluster_wait();
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
-        const uint32_t at = ptx::smem_u32(sums + e);
-        int before = s.next[e], all = 0;
+    ptx::grid_dependency_launch_dependents();
+    for (int x = threadIdx.x; x < q.experts; x += kPlaceThreads) {
+        const uint32_t at = ptx::smem_u32(sums + x);
+        int before = 0, all = 0;
 #pragma unroll
-        for (int r = 0; r < kPlaceCluster; ++r) {
-            const uint32_t from = ptx::mapa_u32(at, r);
+        for (int c = 0; c < kPlaceCluster; ++c) {
+            const uint32_t from = ptx::mapa_u32(at, c);
             before += static_cast<int>(ptx::ld_shared_cluster_u32(from));
             all += static_cast<int>(ptx::ld_shared_cluster_u32(from + q.experts * 4));
         }
-        s.next[e] = before;
-        s.row0[e] = all;
+        s.next[x] += before;
+        if (CHUNKS > 1) next1[x] += before;
+        s.row0[x] = all;
     }
-    ptx::cluster_arrive();      // the others' sums have been read
-    ptx::cluster_wait();        // (what stands in their place next are this CTA's bits)
-    if (chunk >= q.chunks) return;
-    scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
-    if (chunk == 0) write_tables(q, s.row0, s.tile0);
-    const long long first = static_cast<long long>(chunk) * q.chunk_tokens;
-    const int tokens = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - first));
-    place_pairs(q, first * q.top_k, tokens * q.top_k, s.row0, s.tile0, s.next, s.bits);
+    if (pairs <= 0) {
+        __syncthreads();
+        ptx::cluster_arrive_relaxed();
+    } else {
+        scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
+        ptx::cluster_arrive_relaxed();      // (behind a barrier of the CTA: the others' sums have been read)
+        if (chunk == 0) write_tables(q, s.row0, s.tile0);
+        for (int base = 0; base < pairs; base += kAtOnce * kPlaceThreads) {
+            if (base) ask(base);
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+                const int i = base + j * kPlaceThreads + threadIdx.x;
+                if (i < pairs) {
+                    const bool some = e[j] >= 0 && e[j] < q.experts;
+                    put_rows(q, first + i, e[j], some ? (CHUNKS == 1 || i < chunk_pairs ? s.next : next1)[e[j]] + r[j] : 0, s.row0, s.tile0);
+                }
+            }
+        }
+    }
+    ptx::cluster_wait();        // none leaves while its sums are being read
 }
 
-// The rest of a CTA that has counted its chunk's pairs in s.row0: the counts go to the other CTAs, or, where the chunk is the
-// only one, everything is known.
+// The rest of a CTA whose chunk's choices are in global memory: the pairs are counted in s.row0 (zero so far) and ranked.  Where the chunk is the
+// only one this is all; else counts and ranks (in the place of the rows) go to place_kernel.
+//
+// Pairs are ranked 32 * bit_words at a time by a bit per pair and expert, so that the order is that of the pairs whichever
+// thread comes first, and the same expert twice in a token gets two rows.
 __device__ __forceinline__ void finish_chunk(const PlanParams& q, int chunk, const PlanSmem& s) {
-    if (q.chunks > 1) {
+    const long long first = static_cast<long long>(chunk) * q.chunk_tokens * q.top_k;
+    const int pairs = static_cast<int>(min(static_cast<long long>(q.chunk_tokens) * q.top_k, static_cast<long long>(q.tokens) * q.top_k - first));
+    const int words = q.bit_words, batch = 32 * words, stride = words | 1;     // (odd: an expert's words and the next one's in other banks)
+    const bool only = q.chunks == 1;
+    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) s.next[e] = 0;     // pairs ahead of the batch
+    if (pairs > batch && only) {       // the rows need all counts first
+        for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+            const int e = q.expert[first + i];
+            if (e >= 0 && e < q.experts) atomicAdd(&s.row0[e], 1);
+        }
+        __syncthreads();
+        scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
+    }
+    for (int base = 0; base < pairs; base += batch) {
+        const int here = min(batch, pairs - base);
+        for (int i = threadIdx.x; i < q.experts * stride; i += blockDim.x) s.bits[i] = 0u;
+        __syncthreads();
+        for (int i = threadIdx.x; i < here; i += blockDim.x) {
+            const int e = q.expert[first + base + i];
+            if (e >= 0 && e < q.experts) {
+                atomicOr(&s.bits[e * stride + (i >> 5)], 1u << (i & 31));
+                if (!only || pairs <= batch) atomicAdd(&s.row0[e], 1);
+            }
+        }
+        __syncthreads();
+        if (only && pairs <= batch) scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
+        for (int i = threadIdx.x; i < here; i += blockDim.x) {
+            const int e = q.expert[first + base + i];
+            int rank = 0;
+            if (e >= 0 && e < q.experts) {
+                rank = s.next[e] + __popc(s.bits[e * stride + (i >> 5)] & ((1u << (i & 31)) - 1u));
+#pragma unroll 4
+                for (int w = 0; w < (i >> 5); ++w) rank += __popc(s.bits[e * stride + w]);
+            }
+            if (only) put_rows(q, first + base + i, e, rank, s.row0, s.tile0);
+            else q.row[first + base + i] = rank;
+        }
+        if (base + batch >= pairs) break;
+        __syncthreads();
+        for (int e = threadIdx.x; e < q.experts; e += blockDim.x) {
+            int n = 0;
+            for (int w = 0; w < words; ++w) n += __popc(s.bits[e * stride + w]);
+            s.next[e] += n;
+        }
+        __syncthreads();
+    }
+    if (only) write_tables(q, s.row0, s.tile0);
+    else
         for (int e = threadIdx.x; e < q.experts; e += blockDim.x) q.counts[static_cast<long long>(chunk) * counts_row(q.experts) + e] = static_cast<uint16_t>(s.row0[e]);
-        return;
-    }
-    for (int e = threadIdx.x; e < q.experts; e += blockDim.x) s.next[e] = 0;
-    scan_experts(s.row0, s.row0, s.tile0, q.experts, q.tile_shift, s.scratch);
-    write_tables(q, s.row0, s.tile0);
-    place_pairs(q, 0, q.tokens * q.top_k, s.row0, s.tile0, s.next, s.bits);
-}
-
-// Adds a chunk's pairs, given in global memory, to s.row0.
-__device__ __forceinline__ void count_pairs(const PlanParams& q, int chunk, const PlanSmem& s) {
-    const long long first = static_cast<long long>(chunk) * q.chunk_tokens;
-    const int pairs = static_cast<int>(min(static_cast<long long>(q.chunk_tokens), q.tokens - first)) * q.top_k;
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-        const int e = q.expert[first * q.top_k + i];
-        if (e >= 0 && e < q.experts) atomicAdd(&s.row0[e], 1);
-    }
-    __syncthreads();
 }
 
 __global__ void __launch_bounds__(kPlaceThreads) plan_kernel(const PlanParams q) {
@@ -712,7 +749,6 @@ __global__ void __launch_bounds__(kPlaceThreads) plan_kernel(const PlanParams q)
     __syncthreads();
     ptx::grid_dependency_launch_dependents();
     ptx::grid_dependency_wait();
-    count_pairs(q, blockIdx.x, s);
     finish_chunk(q, blockIdx.x, s);
 }
 
@@ -772,7 +808,6 @@ __global__ void __launch_bounds__(route_threads(VPL)) route_kernel(const RoutePa
         ptx::cluster_wait();
         if (rank != 0) return;
     }
-    count_pairs(q, chunk, s);
     finish_chunk(q, chunk, s);
 }
 
