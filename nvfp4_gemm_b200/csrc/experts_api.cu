@@ -33,10 +33,12 @@ int plan_sizes(int tokens, int top_k, int experts, PlanSizes* s) {
     s->max_tiles = pairs / s->tile_tokens + (pairs < experts ? pairs : experts);
     s->sf_rows = s->max_tiles * s->tile_sf_rows;
     if (pairs > 0x7fffffffll || s->sf_rows > 0x7fffffffll) return fail(NVFP4_ERR_INVALID_ARGUMENT, "problem too large: %lld pairs", pairs);
-    // Chunks of the tokens.  Up to 1024 pairs of up to 512 tokens are one: choice and order take one launch.  Else one CTA each, 148 at most
-    // (more only where a chunk's pairs would not be counted in 16 bits).
-    constexpr int kUnit = 8, kMostChunks = 148, kOneChunk = 512, kOneChunkPairs = 1024;
-    const bool one = tokens <= kOneChunk && pairs <= kOneChunkPairs;
+    // Chunks of the tokens: one CTA each, 148 at most (more only where a chunk's pairs would not be counted in 16 bits), or a single one, which
+    // takes one launch for choice and order.  Router, one chunk / more (us): 160 x 8 of 64 experts 6.4 / 7.7, of 256 9.3 / 10.3; 256 x 4 of 32
+    // 6.8 / 7.5; 300 x 2 of 32 7.3 / 7.3; 200 x 6 of 256 11.0 / 10.1 (the pairs of 256 experts are ranked 1152 at a time); 340 x 3 of 64 8.0 / 7.8; 512 x 2 of 64
+    // 8.9 / 7.8; 256 x 8 of 64 9.0 / 7.7.
+    constexpr int kUnit = 8, kMostChunks = 148, kOneChunk = 256;
+    const bool one = tokens <= kOneChunk && pairs <= (experts <= 128 ? 1280 : 1024);
     int chunk_tokens = one ? kOneChunk : kUnit * ((tokens + kUnit * kMostChunks - 1) / (kUnit * kMostChunks));
     if (chunk_tokens < 32) chunk_tokens = 32;
     if (chunk_tokens > kMaxChunkPairs / top_k) chunk_tokens = kMaxChunkPairs / top_k;
@@ -54,16 +56,21 @@ int check_routing(const nvfp4_routing* r, PlanSizes* s) {
     return NVFP4_OK;
 }
 
+// (bits, by which a chunk's pairs are ranked: all of them at once where 36 KB allow it)
+void set_chunks(PlanParams* q, int chunk_tokens, int chunks) {
+    q->chunk_tokens = chunk_tokens;
+    q->chunks = chunks;
+    const int in_chunk = q->tokens < chunk_tokens ? q->tokens : chunk_tokens;
+    const long long needed = (static_cast<long long>(in_chunk) * q->top_k + 31) / 32, most = 9216 / q->experts;
+    q->bit_words = static_cast<int>(needed < most ? needed : most);
+}
+
 PlanParams plan_params(const nvfp4_routing* r, const PlanSizes& s) {
     PlanParams q;
     q.tokens = r->tokens; q.top_k = r->top_k; q.experts = r->experts;
     q.tile_tokens = s.tile_tokens; q.tile_sf_rows = s.tile_sf_rows;
     q.tile_shift = s.tile_tokens == kTileFew ? 5 : 8;
-    q.chunk_tokens = s.chunk_tokens; q.chunks = s.chunks;
-    // all pairs of a chunk at once where 36 KB of bits allow it
-    const int in_chunk = r->tokens < s.chunk_tokens ? r->tokens : s.chunk_tokens;
-    const long long needed = (static_cast<long long>(in_chunk) * r->top_k + 31) / 32, most = 9216 / r->experts;
-    q.bit_words = static_cast<int>(needed < most ? needed : most);
+    set_chunks(&q, s.chunk_tokens, s.chunks);
     q.expert = r->expert; q.row = r->row; q.offset = r->offset;
     int* words = static_cast<int*>(r->plan);
     q.tile_count = words;
@@ -110,8 +117,10 @@ int empty_plan(const PlanParams& q, cudaStream_t stream) {
     return NVFP4_OK;
 }
 
+// More than half of an SM's shared memory: one CTA of the plan's kernels on an SM.  (Two of them, as they come to stand where the kernel ahead leaves
+// SMs free early, share its instructions: 2000 tokens x 8 of 256 18.7 us instead of 17.4, plan of 65536 x 8 of 256 28.8 instead of 21.0.)
 constexpr size_t kPlaceSmem = 116 * 1024;
-constexpr int kPlaceMostCtas = 120;
+constexpr int kPlaceMostCtas = 120;    // as many as 148 SMs hold in clusters of eight
 size_t plan_smem(const PlanParams& q) {
     const int per_expert = (q.bit_words | 1) < 3 ? 3 : (q.bit_words | 1);     // (the place kernel keeps three sums there)
     return (plan_head_words(q.experts) + static_cast<size_t>(q.experts) * per_expert) * sizeof(int);
@@ -271,8 +280,11 @@ int nvfp4_plan_experts(const nvfp4_routing* r, void* stream_v) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
     DeviceCtx* c = nullptr;
     if (int rc = check_device(&c)) return rc;
-    const PlanParams q = plan_params(r, s);
+    PlanParams q = plan_params(r, s);
     if (r->tokens == 0) return empty_plan(q, stream);
+    // Without the choice, how many tokens there are does not count: one chunk / more (us) 200 x 6 of 32 3.9 / 4.2, of 256
+    // 6.3 / 5.4, 350 x 4 of 32 4.2 / 4.4, 384 x 4 of 64 4.5 / 4.5.
+    if (static_cast<long long>(r->tokens) * r->top_k <= (r->experts <= 128 ? 1408 : 1024)) set_chunks(&q, r->tokens, 1);
     const size_t smem = q.chunks > 1 && plan_smem(q) < kPlaceSmem ? kPlaceSmem : plan_smem(q);
     if (int rc = allow_smem(c, 75, reinterpret_cast<const void*>(plan_kernel), smem)) return rc;
     if (int rc = launch(plan_kernel, q.chunks, kPlaceThreads, smem, 1, stream, "plan_experts", q)) return rc;

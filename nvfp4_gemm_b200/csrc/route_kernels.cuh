@@ -183,8 +183,8 @@ __device__ __forceinline__ uint32_t take(Key (&key)[VPL], Key top_key, int lane)
 // apart than the bound allows, the candidates' scores are computed and ranked in 64 bits; where groups are not, the token
 // is chosen again in 64 bits (choose_exactly).
 //
-// Bound by instructions: 8192 tokens of 256 experts take 23.6 us by sigmoid, bias and eight groups, 16.1 by softmax (8.5 of either for the order of the
-// pairs behind it); one token of 64 experts 4.2, of 256 5.2.
+// Bound by instructions: 8192 tokens of 256 experts take 22.1 us by sigmoid, bias and eight groups, 15.0 by softmax (7 of either for the order of the
+// pairs behind it); one token of 64 or 256 experts 3.3 and 3.7.
 //
 // Ranking.  The top_k largest keys are not below the top_k-th largest of the lanes' maxima.  What is not below it, seldom much
 // more than top_k keys, is put side by side, one to a lane, and each counts those ahead of it.  (Taking the largest top_k
@@ -325,8 +325,8 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         for (int i = 0; i < VPL; ++i) key[i] = key_of(x[i]);
     } else {
         // Errors of a score s, in units of 2^-24 of the largest: four for the exponential, one for its argument (times s, at most
-        // 0.37), five for the quotient, VPL + 5 for the softmax's total; then one of the choice.  Two compared values of two scores
-        // each: four times that.
+        // 0.37), five for the quotient, VPL + 5 for the softmax's total; then one of the choice.  Two compared choices: twice that;
+        // groups' sums of two: four times, and the roundings of the sums.
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             // (an expert whose logit or bias is -inf or NaN: -inf)
@@ -334,7 +334,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             key[i] = key_of(c);
         }
         const float units = p.scoring == kScoreSoftmax ? __fdividef(VPL + 16.f, total) : 10.f;      // (the largest softmax score is 1 / total)
-        apart = 4.f * 5.9604645e-8f * (units + most);
+        apart = 2.f * 5.9604645e-8f * (units + most);
     }
     if (p.groups > 1) {
         // A group's experts are those of direct_lanes neighbouring lanes; or, where lanes hold experts of several groups, the keys go through
@@ -383,7 +383,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         if constexpr (!BY_LOGIT) {
             const uint32_t worst = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu);
             const uint32_t best = __reduce_max_sync(0xffffffffu, keep || g >= p.groups ? 0u : mine);
-            if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > apart)) apart = INFINITY;
+            if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > 2.f * apart + 4.f * 5.9604645e-8f * most)) apart = INFINITY;
         }
         if (direct) {
 #pragma unroll
@@ -405,6 +405,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
     int n = 0, rank = 0;
     uint32_t mine = 0u;
     expert = -1;
+    bool tight = false;         // the candidates may not be all that are too near to the last one to be told apart
     if constexpr (VPL == 1) {
         mine = key[0];
         expert = lane;
@@ -426,36 +427,43 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             ahead += (o.x > best) + (o.y > best) + (o.z > best) + (o.w > best);
         }
         uint32_t floor_key = least > 32 ? 0u : __reduce_min_sync(0xffffffffu, ahead < least ? best : 0xffffffffu);
-        if (floor_key == 0) {
-            // Fewer lanes than that have anything (few groups or experts are left, a lane's experts are neighbours): the least-th largest
-            // key itself, from one value to the next.
-            // (8192 tokens, two of eight groups of 256 experts: 29 us; all of them a candidate, more than lanes, and chosen in 64 bits: 56)
-            int keys_left = 0;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) keys_left += __popc(__ballot_sync(0xffffffffu, key[i] != 0));
-            uint32_t above = 0xffffffffu;
-            for (int left = keys_left > 32 ? least : 0; left > 0;) {
-                uint32_t next = 0u;
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) next = max(next, key[i] < above ? key[i] : 0u);
-                next = warp_max(next);
-                if (next == 0) break;
-#pragma unroll
-                for (int i = 0; i < VPL; ++i) left -= __popc(__ballot_sync(0xffffffffu, key[i] == next));
-                floor_key = above = next;
-            }
-        }
         if (!BY_LOGIT && floor_key) floor_key = key_of(value_of(floor_key) - apart);
         floor_key = max(floor_key, 1u);
         __syncwarp();
         cand[lane] = 0u;
         __syncwarp();
         int pos = 0;        // candidates of the lanes ahead: side by side in the order of the experts
+        auto count_candidates = [&]() {
+            n = pos = 0;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-            const uint32_t b = __ballot_sync(0xffffffffu, key[i] >= floor_key);
-            pos += __popc(b & ((1u << lane) - 1u));
-            n += __popc(b);
+            for (int i = 0; i < VPL; ++i) {
+                const uint32_t b = __ballot_sync(0xffffffffu, key[i] >= floor_key);
+                pos += __popc(b & ((1u << lane) - 1u));
+                n += __popc(b);
+            }
+        };
+        count_candidates();
+        if (n > 32 && least <= 32 && !unsure_group) {
+            // More than lanes: fewer lanes have anything than are to be chosen (few groups or experts are left, a lane's experts are neighbours), or
+            // nearly as many are to be chosen as there are lanes.  A threshold that `least` to 32 keys are not below, by halves.
+            // (8192 tokens of 256 experts: 2 of 8 groups by logits 17.4 us, chosen in 64 bits 56; 24 and 32 of all 21.5 and 24.6, in 64 bits 53 and 64)
+            uint32_t low = floor_key, high = warp_max(best);      // more than 32 are not below low; fewer than least above high
+#pragma unroll 1
+            while (low < high) {
+                const uint32_t mid = low + (high - low + 1) / 2;
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) c += key[i] >= mid;
+                c = __reduce_add_sync(0xffffffffu, c);
+                if (c > 32) low = mid;
+                else if (c < least) high = mid - 1;
+                else {
+                    floor_key = mid;
+                    tight = true;
+                    break;
+                }
+            }
+            if (tight) count_candidates();
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
@@ -468,19 +476,18 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         rank = rank_of(mine, lane, cand, min(n, 32));
     }
     float logit = 0.f;
-    if (n > 32 || unsure_group) {
-        // more alike than lanes, or groups that 32 bits cannot tell apart
-        __syncwarp();
-        n = choose_exactly<BY_LOGIT, VPL>(p, q, token, lane, reinterpret_cast<uint64_t*>(keys), expert, logit);
-        slot = expert >= 0 ? lane : -1;
-    } else {
+    bool by_hand = n > 32 || unsure_group;
+    if (!by_hand) {
         if constexpr (!BY_LOGIT) {
             uint32_t* const sorted = keys + 64;
             if (mine) sorted[rank] = mine;
             __syncwarp();
             bool sure = true;
             if (lane < q.top_k && lane + 1 < n) sure = value_of(sorted[lane]) - value_of(sorted[lane + 1]) > apart;
-            if (!__all_sync(0xffffffffu, sure)) {
+            const bool all_sure = __all_sync(0xffffffffu, sure);
+            // (candidates by halves hold at least one more than are chosen: those that may be chosen, if the last is sure to be none of them)
+            by_hand = !all_sure && tight && !(value_of(sorted[q.top_k - 1]) - value_of(sorted[n - 1]) > apart);
+            if (!all_sure && !by_hand) {
                 double all = 1.0;
                 if (p.scoring == kScoreSoftmax) {
                     all = 0.0;
@@ -502,6 +509,12 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         }
         slot = mine && rank < q.top_k ? rank : -1;
         if (slot >= 0) logit = BY_LOGIT ? value_of(mine) : load_logit(p, token * p.logits_row_stride + expert);
+    }
+    if (by_hand) {
+        // more alike than lanes, or groups that 32 bits cannot tell apart
+        __syncwarp();
+        n = choose_exactly<BY_LOGIT, VPL>(p, q, token, lane, reinterpret_cast<uint64_t*>(keys), expert, logit);
+        slot = expert >= 0 ? lane : -1;
     }
     float s = 0.f;
     if (slot >= 0) {
@@ -587,7 +600,8 @@ struct PlanSmem {
 // One or two chunks' share of the order, where the counts of all chunks (16 bits each) and every pair's rank in its chunk are known.  The eight CTAs of a
 // cluster share the work of adding the counts up: each sums every eighth chunk, over all chunks and over those ahead of the cluster's, and takes the
 // others' sums from their shared memory.  (Each CTA for itself: 148 CTAs read the same 75 KB of 256 experts' counts in 8000 cycles.)
-// Two chunks where one each would be more CTAs than clusters of eight find room for at one CTA an SM (TWO_US).
+// Two chunks where one each would be more CTAs than clusters of eight find room for at one CTA an SM (choice and order of 8192 x 8 of 256, softmax: 14.9 us, 17.3
+// with one).
 constexpr int kPlaceCluster = 8;
 template <int CHUNKS>
 __global__ void __launch_bounds__(kPlaceThreads, 1) place_kernel(const PlanParams q) {

@@ -552,3 +552,40 @@ def test_choices_from_few_groups(ex, lib, experts, groups, top_groups, top_k, kw
         pytest.skip("fewer experts in the groups than choices")
     r = ex.route(x.cuda(), top_k, **{**kw, **({"bias": kw["bias"].cuda()} if "bias" in kw else {})})
     _check_routing(lib, r, x, top_k, experts, **kw)
+
+
+@pytest.mark.parametrize("experts,top_k", [(64, 24), (64, 32), (256, 20), (256, 31), (256, 32), (384, 28), (1024, 32)])
+@pytest.mark.parametrize("kw", [dict(), dict(scoring="sigmoid", bias=True), dict(bias=True, groups=4, top_groups=3, group_score="top2")], ids=str)
+def test_nearly_as_many_choices_as_lanes(ex, lib, experts, top_k, kw):
+    g = _gen(experts + top_k)
+    x = torch.randn((70, experts), generator=g)
+    x[3] = x[3].bfloat16()           # ties
+    x[4, 40:] = -INF
+    x[5] = 0.25                      # all alike
+    kw = dict(kw)
+    if kw.get("bias"):
+        kw["bias"] = torch.randn(experts, generator=g) * 0.2
+    r = ex.route(x.cuda(), top_k, **{**kw, **({"bias": kw["bias"].cuda()} if "bias" in kw else {})})
+    _check_routing(lib, r, x, top_k, experts, **kw)
+
+
+@pytest.mark.parametrize("size", [1.0, 64.0, 4096.0])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+def test_biases_that_outweigh_the_scores(ex, lib, size, scoring):
+    """Choices whose 32-bit sums show little or nothing of the scores that tell them apart, those of the groups among them."""
+    g = _gen(5)
+    x = torch.randn((300, 256), generator=g)
+    bias = torch.full((256,), size)
+    bias[::7] += size / 64
+    kw = dict(scoring=scoring, groups=8, top_groups=3, group_score="top2")
+    r = ex.route(x.cuda(), 8, bias=bias.cuda(), **kw)
+    _check_routing(lib, r, x, 8, 256, bias=bias, **kw)
+
+
+@pytest.mark.parametrize("tokens,top_k,experts", [(176, 8, 32), (177, 8, 32), (352, 4, 128), (128, 8, 129), (256, 5, 128), (257, 5, 128), (161, 8, 64), (3900, 3, 16), (4000, 9, 300)])
+def test_plans_about_the_borders_of_one_chunk_and_of_two_chunks_a_cta(ex, tokens, top_k, experts):
+    g = _gen(tokens)
+    ids = torch.randint(-1, experts + 1, (tokens, top_k), generator=g, dtype=torch.int32)       # repeated, and some that are none
+    for r in (ex.plan(ids.cuda(), experts), ex.plan((ids * 0 + experts // 2).cuda(), experts)):
+        rows, offsets = ref.order(r.experts.cpu(), experts)
+        assert torch.equal(r.rows.cpu(), rows) and torch.equal(r.offsets.cpu(), offsets)
