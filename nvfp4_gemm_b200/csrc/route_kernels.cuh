@@ -401,14 +401,17 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
     // candidates, one to a lane: cand holds their keys, ids their experts
     uint32_t* const cand = keys;
     uint32_t* const ids = keys + 32;
+    [[maybe_unused]] float* const logits = reinterpret_cast<float*>(keys + 96);       // (those of the scores' candidates)
     const bool unsure_group = !BY_LOGIT && apart == INFINITY;
     int n = 0, rank = 0;
     uint32_t mine = 0u;
     expert = -1;
     bool tight = false;         // the candidates may not be all that are too near to the last one to be told apart
+    float logit = 0.f;
     if constexpr (VPL == 1) {
         mine = key[0];
         expert = lane;
+        logit = x[0];
         cand[lane] = mine;
         n = __popc(__ballot_sync(0xffffffffu, mine != 0));
         __syncwarp();
@@ -468,14 +471,21 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
             if (key[i] >= floor_key) {
-                if (pos < 32) { cand[pos] = key[i]; ids[pos] = lane * VPL + i; }
+                if (pos < 32) {
+                    cand[pos] = key[i];
+                    ids[pos] = lane * VPL + i;
+                    if (!BY_LOGIT) logits[pos] = x[i];
+                }
                 ++pos;
             }
         __syncwarp();
-        if (lane < n) { mine = cand[lane]; expert = ids[lane]; }
+        if (lane < n) {
+            mine = cand[lane];
+            expert = ids[lane];
+            if (!BY_LOGIT) logit = logits[lane];
+        }
         rank = rank_of(mine, lane, cand, min(n, 32));
     }
-    float logit = 0.f;
     bool by_hand = n > 32 || unsure_group;
     if (!by_hand) {
         if constexpr (!BY_LOGIT) {
@@ -497,18 +507,19 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
                 }
                 uint64_t exact = 0;
                 if (mine) {
-                    const double l = load_logit(p, token * p.logits_row_stride + expert);
+                    const double l = logit;
                     exact = key_of((p.scoring == kScoreSoftmax ? exp(l - top) / all : 1.0 / (1.0 + exp(-l))) + (p.bias ? static_cast<double>(p.bias[expert]) : 0.0));
                 }
                 rank = 0;
-                for (int j = 0; j < 32; ++j) {
+#pragma unroll 4
+                for (int j = 0; j < (VPL == 1 ? 32 : n); ++j) {
                     const uint64_t other = __shfl_sync(0xffffffffu, exact, j);
                     rank += other > exact || (other == exact && j < lane);
                 }
             }
         }
         slot = mine && rank < q.top_k ? rank : -1;
-        if (slot >= 0) logit = BY_LOGIT ? value_of(mine) : load_logit(p, token * p.logits_row_stride + expert);
+        if (BY_LOGIT && slot >= 0) logit = value_of(mine);
     }
     if (by_hand) {
         // more alike than lanes, or groups that 32 bits cannot tell apart
