@@ -269,6 +269,21 @@ __device__ __noinline__ int choose_exactly(const RouteParams& p, const PlanParam
     return n;
 }
 
+// A choice in 64 bits.  all: sum of exp(x - top) over the experts (softmax).
+__device__ __forceinline__ double exact_choice(int scoring, float x, float top, double all, float bias) {
+    const double l = x;
+    return (scoring == kScoreSoftmax ? exp(l - top) / all : 1.0 / (1.0 + exp(-l))) + static_cast<double>(bias);
+}
+// (for loops that stand unrolled)
+__device__ __noinline__ double exact_choice_call(int scoring, float x, float top, double all, float bias) { return exact_choice(scoring, x, top, all, bias); }
+template <int VPL>
+__device__ __forceinline__ double exact_total(const float (&x)[VPL], float top) {
+    double all = 0.0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) all += x[i] == -INFINITY ? 0.0 : exp(static_cast<double>(x[i]) - top);
+    return warp_sum(all);
+}
+
 // Rank of this lane's key among `of` keys of shared memory (16-byte aligned, the last four filled up with zeros): larger ones, and
 // as large ones of a lower place.
 __device__ __forceinline__ int rank_of(uint32_t mine, int place, const uint32_t* of, int count) {
@@ -333,7 +348,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             const float c = fmaxf(x[i] == -INFINITY ? -INFINITY : t[i] + bias[i], -INFINITY);
             key[i] = key_of(c);
         }
-        const float units = p.scoring == kScoreSoftmax ? __fdividef(VPL + 16.f, total) : 10.f;      // (the largest softmax score is 1 / total)
+        const float units = p.scoring == kScoreSoftmax ? __fdividef(VPL + 16.f, fmaxf(total, 1.f)) : 10.f;      // (the largest softmax score is 1 / total, and total 0 where nothing can be chosen)
         apart = 2.f * 5.9604645e-8f * (units + most);
     }
     if (p.groups > 1) {
@@ -379,11 +394,45 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             const uint32_t other = __shfl_sync(0xffffffffu, mine, h * lanes);
             rank += other > mine || (other == mine && h < g);
         }
-        const bool keep = g < p.groups && rank < p.top_groups;
+        bool keep = g < p.groups && rank < p.top_groups;
         if constexpr (!BY_LOGIT) {
             const uint32_t worst = __reduce_min_sync(0xffffffffu, keep ? mine : 0xffffffffu);
             const uint32_t best = __reduce_max_sync(0xffffffffu, keep || g >= p.groups ? 0u : mine);
-            if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > 2.f * apart + 4.f * 5.9604645e-8f * most)) apart = INFINITY;
+            const float margin = 2.f * apart + 4.f * 5.9604645e-8f * most;
+            if (best != 0 && worst != 0 && !(value_of(worst) - value_of(best) > margin)) {
+                if (!direct) {
+                    apart = INFINITY;
+                } else {
+                    // Groups that are that near to the border compete for the places there with scores of 64 bits, made of the choices that may
+                    // be their largest (one such token in 8192 cost 2.5 us of the launch when it was chosen again as a whole).
+                    const bool open = g < p.groups && (keep ? !(value_of(mine) - value_of(best) > margin) : !(value_of(worst) - value_of(mine) > margin));
+                    const uint32_t last = p.group_top == 2 ? second : first;
+                    const uint32_t from = last ? max(key_of(value_of(last) - apart), 1u) : 1u;
+                    double all = 1.0, e1 = -INFINITY, e2 = -INFINITY;
+                    if (p.scoring == kScoreSoftmax) all = exact_total<VPL>(x, top);
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i)
+                        if (open && key[i] >= from) {
+                            const double c = exact_choice_call(p.scoring, x[i], top, all, bias[i]);
+                            e2 = fmax(e2, fmin(e1, c));
+                            e1 = fmax(e1, c);
+                        }
+                    for (int s = 1; s < lanes; s <<= 1) {
+                        const double f = __shfl_xor_sync(0xffffffffu, e1, s), u = __shfl_xor_sync(0xffffffffu, e2, s);
+                        e2 = fmax(fmin(e1, f), fmax(e2, u));
+                        e1 = fmax(e1, f);
+                    }
+                    const double score = p.group_top == 2 && e2 != -INFINITY ? e1 + e2 : e1;
+                    const uint32_t opened = __ballot_sync(0xffffffffu, open);
+                    const int places = __popc(__ballot_sync(0xffffffffu, open && keep && (lane & (lanes - 1)) == 0));
+                    int ahead = 0;
+                    for (int h = 0; h < p.groups; ++h) {
+                        const double other = __shfl_sync(0xffffffffu, score, h * lanes);
+                        ahead += (opened >> (h * lanes) & 1u) && (other > score || (other == score && h < g));
+                    }
+                    if (open) keep = ahead < places;
+                }
+            }
         }
         if (direct) {
 #pragma unroll
@@ -498,18 +547,9 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
             // (candidates by halves hold at least one more than are chosen: those that may be chosen, if the last is sure to be none of them)
             by_hand = !all_sure && tight && !(value_of(sorted[q.top_k - 1]) - value_of(sorted[n - 1]) > apart);
             if (!all_sure && !by_hand) {
-                double all = 1.0;
-                if (p.scoring == kScoreSoftmax) {
-                    all = 0.0;
-#pragma unroll
-                    for (int i = 0; i < VPL; ++i) all += x[i] == -INFINITY ? 0.0 : exp(static_cast<double>(x[i]) - top);
-                    all = warp_sum(all);
-                }
+                const double all = p.scoring == kScoreSoftmax ? exact_total<VPL>(x, top) : 1.0;
                 uint64_t exact = 0;
-                if (mine) {
-                    const double l = logit;
-                    exact = key_of((p.scoring == kScoreSoftmax ? exp(l - top) / all : 1.0 / (1.0 + exp(-l))) + (p.bias ? static_cast<double>(p.bias[expert]) : 0.0));
-                }
+                if (mine) exact = key_of(exact_choice(p.scoring, logit, top, all, p.bias ? p.bias[expert] : 0.f));
                 rank = 0;
 #pragma unroll 4
                 for (int j = 0; j < (VPL == 1 ? 32 : n); ++j) {

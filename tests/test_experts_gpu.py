@@ -589,3 +589,26 @@ def test_plans_about_the_borders_of_one_chunk_and_of_two_chunks_a_cta(ex, tokens
     for r in (ex.plan(ids.cuda(), experts), ex.plan((ids * 0 + experts // 2).cuda(), experts)):
         rows, offsets = ref.order(r.experts.cpu(), experts)
         assert torch.equal(r.rows.cpu(), rows) and torch.equal(r.offsets.cpu(), offsets)
+
+
+@pytest.mark.parametrize("experts,groups", [(256, 8), (64, 4), (1024, 16), (160, 8)])
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+def test_groups_at_the_border_of_what_32_bits_tell_apart(ex, lib, experts, groups, scoring, group_score):
+    """Groups of the same logits in another order, but for one bit of one of them: equal, or apart by less than 32 bits show of a score."""
+    g = _gen(experts)
+    per, tokens = experts // groups, 60
+    one = torch.randn((tokens, 1, per), generator=g)
+    x = torch.stack([one[:, 0, torch.randperm(per, generator=g)] for _ in range(groups)], 1).contiguous()
+    for t in range(tokens):
+        for h in torch.randperm(groups, generator=g)[:groups // 2].tolist():
+            at = x[t, h].topk(3).indices[t % 3]          # the largest, the second, or one that does not count
+            x[t, h, at] = torch.nextafter(x[t, h, at], torch.tensor(INF if t % 2 else -INF))
+    x[1, 0] = -INF                                       # groups with one expert and with none
+    x[2, 1, 1:] = -INF
+    x = x.view(tokens, experts)
+    kw = dict(scoring=scoring, groups=groups, top_groups=groups // 2, group_score=group_score)
+    bias = torch.full((experts,), 0.125)
+    for more in (dict(), dict(bias=bias)):
+        r = ex.route(x.cuda(), 6, **kw, **{k: v.cuda() for k, v in more.items()})
+        _check_routing(lib, r, x, 6, experts, **kw, **more)
