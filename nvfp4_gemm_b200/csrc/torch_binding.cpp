@@ -304,8 +304,9 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
 
 PyObject* status_object(int rc) { return PyLong_FromLong(rc); }
 
-PyObject* pack(std::initializer_list<at::Tensor> tensors) {
-    PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+// (a number, if given, behind the tensors)
+PyObject* pack(std::initializer_list<at::Tensor> tensors, int64_t number = -1) {
+    PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()) + (number >= 0));
     if (!out) throw PythonError{};
     Py_ssize_t i = 0;
     for (const at::Tensor& t : tensors) {
@@ -315,6 +316,14 @@ PyObject* pack(std::initializer_list<at::Tensor> tensors) {
             throw PythonError{};
         }
         PyTuple_SET_ITEM(out, i++, o);
+    }
+    if (number >= 0) {
+        PyObject* o = PyLong_FromLongLong(number);
+        if (!o) {
+            Py_DECREF(out);
+            throw PythonError{};
+        }
+        PyTuple_SET_ITEM(out, i, o);
     }
     return out;
 }
@@ -379,7 +388,7 @@ double float_arg(PyObject* o) {
     return v;
 }
 
-// route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan)
+// route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan, number of experts)
 PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return guarded([&]() -> PyObject* {
         if (nargs != 9) raise(PyExc_TypeError, "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale)");
@@ -412,7 +421,7 @@ PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         o.logits_row_stride = row_stride(logits);
         o.weights = routing.weight.data_ptr<float>();
         const int rc = on_current_stream(logits, [&](void* stream) { return nvfp4_route(&o, &routing.r, stream); });
-        return rc ? status_object(rc) : pack({routing.expert, routing.weight, routing.row, routing.offset, routing.plan});
+        return rc ? status_object(rc) : pack({routing.expert, routing.weight, routing.row, routing.offset, routing.plan}, logits.size(1));
     });
 }
 
@@ -589,7 +598,7 @@ PyMethodDef methods[] = {
     {"gemm_epilogue", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_gemm_epilogue)), METH_FASTCALL,
      "gemm_epilogue(data, bias, activation, out, tile_n, grid, cta_group, split_k[, residual]) -> status"},
     {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_route)), METH_FASTCALL,
-     "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan) or status"},
+     "route(logits, top_k, scoring, bias, groups, top_groups, group_top, renormalize, scale) -> (experts, weights, rows, offsets, plan, number of experts) or status"},
     {"plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_plan)), METH_FASTCALL, "plan(experts, number of experts) -> (rows, offsets, plan) or status"},
     {"quantize_routed", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_quantize_routed)), METH_FASTCALL,
      "quantize_routed(x, rows, plan, number of experts) -> (packed, sf) or status"},

@@ -9,7 +9,7 @@ or all of it in one call, :func:`expert_layer`.  Between the router and the comb
 (token, choice), in expert order: by expert, within an expert by token.  ``w`` [N, K/2, E] and ``w_sf``
 [32, 4, N/128, 4, K/64, E] are laid out like ``b`` and ``sfb_permuted`` of :func:`submission.custom_kernel` with one batch entry per
 expert.  Everything is enqueued on torch's current stream of the tensors' device and not waited for; nothing is kept
-between calls.  All compute is in the CUDA library behind the C ABI; there is no PyTorch or CPU path.  The reference has one
+between calls.  All compute is in the CUDA library behind the C ABI; there is no PyTorch or CPU path, and no gradient.  The reference has one
 dense product and no counterpart.
 """
 from __future__ import annotations
@@ -64,8 +64,11 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: O
     scores without bias, divided by their sum if ``renormalize`` (0 where that is 0), times ``scale``.
     An expert whose logit or bias is -inf or NaN cannot be chosen; a token with fewer than ``top_k`` others gets expert -1,
     row -1 and weight 0 for the rest, so a padded token is one whose logits are all -inf.  Choices are made in 64 bits."""
-    return Routing(*_checked(_lib.native().route(logits, top_k, _choice(_SCORING, scoring, "scoring"), bias, groups, top_groups,
-                                                 _choice(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), scale)), logits.shape[1])
+    result = _lib.native().route(logits, top_k, _SCORING.get(scoring) or _choice(_SCORING, scoring, "scoring"), bias, groups, top_groups,
+                                 _GROUP_SCORE.get(group_score) or _choice(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), scale)
+    if type(result) is int:
+        _lib.check(result)
+    return tuple.__new__(Routing, result)
 
 
 def plan(experts: torch.Tensor, num_experts: int) -> Routing:
