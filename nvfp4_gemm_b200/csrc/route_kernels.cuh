@@ -94,7 +94,7 @@ __device__ __forceinline__ double warp_sum(double v) {
 }
 
 // A logit as the router sees it: NaN and -inf mark an expert that cannot be chosen, +inf counts as the largest number.
-__device__ __forceinline__ float as_logit(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
+__device__ __forceinline__ float as_logit(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }      // (the larger of NaN and a number is the number)
 __device__ __forceinline__ float load_logit(const RouteParams& p, long long at) {
     if (p.logit_type == kLogitFp32) return as_logit(static_cast<const float*>(p.logits)[at]);
     if (p.logit_type == kLogitBf16) return as_logit(__bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]));
@@ -154,9 +154,11 @@ __device__ __forceinline__ void as_logits(const RouteParams& p, int lane, int ex
 #pragma unroll
         for (int i = 0; i < VPL; ++i) x[i] = as_logit(__half2float(__ushort_as_half(static_cast<unsigned short>(raw[i]))));
     }
+    if (experts != 32 * VPL) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-        if (lane * VPL + i >= experts) x[i] = -INFINITY;
+        for (int i = 0; i < VPL; ++i)
+            if (lane * VPL + i >= experts) x[i] = -INFINITY;
+    }
 }
 
 // Takes the key out of the warp's keys that is top_key, the one of the lowest expert where several are: that expert.  (Each key is compared
