@@ -182,11 +182,12 @@ __device__ __forceinline__ uint32_t take(Key (&key)[VPL], Key top_key, int lane)
 // are those of the logits, and exact.  Otherwise two scores may be nearer to each other than 32 bits show, and which
 // experts are taken must not depend on how an exponential rounds.  The scores are computed in 32 bits all the same, with a
 // bound on their error, and every decision is checked against it: where two neighbours of the ranking are not further
-// apart than the bound allows, the candidates' scores are computed and ranked in 64 bits; where groups are not, the token
-// is chosen again in 64 bits (choose_exactly).
+// apart than the bound allows, the candidates' scores are computed and ranked in 64 bits; where groups are not, theirs
+// are, or (groups whose experts are not those of whole lanes) the token is chosen again in 64 bits (choose_exactly).  A launch waits
+// for its slowest token, so these paths count although few tokens take them.
 //
-// Bound by instructions: 8192 tokens of 256 experts take 22.1 us by sigmoid, bias and eight groups, 15.0 by softmax (7 of either for the order of the
-// pairs behind it); one token of 64 or 256 experts 3.3 and 3.7.
+// Bound by instructions (1200 a token of 256 experts, 2.2 a cycle and SM): 8192 tokens of 256 experts take 20.0 us by sigmoid, bias and eight groups, 15.0 by
+// softmax (5 of either for the order of the pairs behind it); one token of 64 or 256 experts 3.3 and 3.7.
 //
 // Ranking.  The top_k largest keys are not below the top_k-th largest of the lanes' maxima.  What is not below it, seldom much
 // more than top_k keys, is put side by side, one to a lane, and each counts those ahead of it.  (Taking the largest top_k
