@@ -376,9 +376,9 @@ typedef struct nvfp4_expert_problem {
     const void* bias;       /* fp16 [experts][n] or NULL */
     int32_t n, k;
     int64_t a_row_stride;                     /* bytes */
-    int64_t w_row_stride, w_expert_stride;    /* bytes */
-    int64_t sfw_perm_expert_stride;           /* bytes */
-    int64_t bias_expert_stride;               /* elements */
+    int64_t w_row_stride, w_expert_stride;    /* bytes; experts do not share weights (at least k / 2 apart) */
+    int64_t sfw_perm_expert_stride;           /* bytes (at least 512) */
+    int64_t bias_expert_stride;               /* elements; 0: one bias for all */
     int32_t activation;     /* NVFP4_ACT_* */
     int32_t output;         /* NVFP4_OUT_* */
     float out_scale;

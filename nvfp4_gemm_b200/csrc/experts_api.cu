@@ -342,9 +342,10 @@ int nvfp4_expert_gemm(const nvfp4_expert_problem* p, const nvfp4_routing* r, voi
     const int n_out = p->activation == NVFP4_ACT_SWIGLU ? p->n / 2 : p->n;
     if (p->a_row_stride % 16 || p->w_row_stride % 16 || p->a_row_stride < p->k / 2 || p->w_row_stride < p->k / 2)
         return fail(NVFP4_ERR_INVALID_ARGUMENT, "row strides of a and w must be multiples of 16 bytes and >= k/2");
-    if (r->experts > 1 && (p->w_expert_stride % 16 || p->sfw_perm_expert_stride % 16 || p->w_expert_stride < 0 || p->sfw_perm_expert_stride < 0 ||
+    // (the bias may be one for all; weights that several experts share cannot be described to tensor loads)
+    if (r->experts > 1 && (p->w_expert_stride % 16 || p->sfw_perm_expert_stride % 16 || p->w_expert_stride < p->k / 2 || p->sfw_perm_expert_stride < 512 ||
                            (p->bias && p->bias_expert_stride < 0)))
-        return fail(NVFP4_ERR_INVALID_ARGUMENT, "expert strides must not be negative and keep 16-byte alignment");
+        return fail(NVFP4_ERR_INVALID_ARGUMENT, "expert strides must keep 16-byte alignment and the experts' weights and scales apart, the bias's must not be negative");
     if (to_nvfp4 ? (p->out_row_stride % 16 || p->out_row_stride < n_out / 2) : (p->out_row_stride % 8 || p->out_row_stride < n_out))
         return fail(NVFP4_ERR_INVALID_ARGUMENT, "out_row_stride must keep 16-byte alignment and hold a row");
     DeviceCtx* c = nullptr;

@@ -79,6 +79,11 @@ def test_grouped_product_refusals(lib, over, text):
     _refused(lib, lib.nvfp4_expert_gemm(_problem(**over), _routing(), None), text)
 
 
+@pytest.mark.parametrize("over", [dict(w_expert_stride=0), dict(sfw_perm_expert_stride=0), dict(w_expert_stride=16), dict(bias_expert_stride=-8)])
+def test_experts_that_share_weights_are_refused(lib, over):
+    _refused(lib, lib.nvfp4_expert_gemm(_problem(bias=A, **over), _routing(), None), "expert strides")
+
+
 @pytest.mark.parametrize("args,text", [
     (dict(k=96), "multiple of 64"), (dict(x=None), "must not be NULL"), (dict(x=A + 8), "16-byte aligned"), (dict(stride=252), "row stride"),
     (dict(packed=A + 4), "packed"), (dict(packed_stride=100), "packed"), (dict(sf=A + 8), "16-byte aligned"),

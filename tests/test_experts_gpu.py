@@ -612,3 +612,16 @@ def test_groups_at_the_border_of_what_32_bits_tell_apart(ex, lib, experts, group
     for more in (dict(), dict(bias=bias)):
         r = ex.route(x.cuda(), 6, **kw, **{k: v.cuda() for k, v in more.items()})
         _check_routing(lib, r, x, 6, experts, **kw, **more)
+
+
+def test_one_bias_for_all_experts(ex, lib):
+    g = _gen(8)
+    experts, n, k, top_k = 4, 128, 256, 2
+    x = torch.randn((30, k), generator=g).half().cuda()
+    r = ex.route(torch.randn((30, experts), generator=g).cuda(), top_k)
+    w = torch.randint(0, 256, (experts, n, k // 2), generator=g, dtype=torch.uint8).cuda().permute(1, 2, 0)
+    w_sf = torch.full((experts, n // 128, k // 64, 32, 4, 4), 0x38, dtype=torch.uint8, device="cuda").permute(3, 4, 1, 5, 2, 0)
+    one = torch.randn((1, n), generator=g).half().cuda()
+    rows = ex.quantize_routed(x, r)
+    y = ex.expert_gemm(rows, r, w, w_sf, bias=one.expand(experts, n))
+    assert torch.equal(y, ex.expert_gemm(rows, r, w, w_sf, bias=one.repeat(experts, 1)))
