@@ -1,4 +1,4 @@
-"""The mixture-of-experts operators in 64 bits, written for reading (checker, never the thing under test)."""
+"""The mixture-of-experts operators in 64 bits, written for reading (what the kernels are compared with)."""
 import math
 
 import torch
