@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
                 } else {
                     if (p.activation == kExpertRelu) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) z[i] = fmaxf(z[i], 0.f);
+                        for (int i = 0; i < 32; ++i) z[i] = ptx::relu(z[i]);
                     } else if (p.activation == kExpertSilu) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) z[i] = __fdividef(z[i], 1.f + __expf(-z[i]));

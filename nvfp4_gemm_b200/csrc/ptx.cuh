@@ -79,6 +79,13 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
     return ok != 0;
 }
 
+// max(x, 0) that keeps a NaN (fmaxf answers with the number).
+__device__ __forceinline__ float relu(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // Programmatic dependent launch.  launch_dependents: the next kernel in the stream (if it was
 // launched with programmatic stream serialisation) may be scheduled once every CTA of this grid
 // has said so or exited.  wait: everything the stream ordered before this grid has completed
