@@ -97,7 +97,7 @@ int nvfp4_gemm(const nvfp4_problem* problem, const nvfp4_gemm_config* cfg, void*
  * The reference writes fp16 only (sub_cub.py:98-104, s_128t.py:324-359); no counterpart.
  */
 #define NVFP4_ACT_NONE 0
-#define NVFP4_ACT_RELU 1
+#define NVFP4_ACT_RELU 1    /* max(x, 0); a NaN stays one, here and in the experts' product */
 #define NVFP4_ACT_SILU 2
 #define NVFP4_OUT_FP16 0
 #define NVFP4_OUT_NVFP4 1

@@ -285,7 +285,7 @@ __device__ __forceinline__ void add_fp16x16(const uint4 (&r)[2], float* s) {
 __device__ __forceinline__ void activate16(int activation, float* s) {
     if (activation == kActRelu) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fmaxf(s[i], 0.f);
+        for (int i = 0; i < 16; ++i) s[i] = ptx::relu(s[i]);
     } else if (activation == kActSilu) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = __fdividef(s[i], 1.f + __expf(-s[i]));
