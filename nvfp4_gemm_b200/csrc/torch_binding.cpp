@@ -201,6 +201,7 @@ PyObject* py_gemm_epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
         nvfp4_epilogue e;
         std::memset(&e, 0, sizeof(e));
         if (const at::Tensor* bias = tensor_or_none(args[1])) {
+            if (bias->device() != o.t[0]->device()) raise(PyExc_ValueError, "bias must be on the device of a");
             if (bias->scalar_type() != at::kHalf || bias->numel() != p.n || !bias->is_contiguous())
                 raise(PyExc_ValueError, "bias must be a contiguous fp16 vector of length n");
             e.bias = bias->data_ptr();
