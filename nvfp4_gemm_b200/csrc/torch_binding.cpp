@@ -214,13 +214,17 @@ PyObject* py_gemm_epilogue(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
             } const out{PySequence_Fast(args[3], "out must be (packed, sf, sf_permuted)")};
             if (!out.seq) throw PythonError{};
             if (PySequence_Fast_GET_SIZE(out.seq) < 3) raise(PyExc_IndexError, "out must be (packed, sf, sf_permuted)");
+            const int64_t m = p.m, n = p.n;
+            const int64_t needed[3] = {p.l * m * (n / 2), p.l * m * (n / 16), p.l * ((m + 127) / 128) * (n / 64) * 512};
             void* ptr[3];
             for (int i = 0; i < 3; ++i) {
                 const at::Tensor* t = tensor_or_none(PySequence_Fast_GET_ITEM(out.seq, i));
                 if (!t) raise(PyExc_TypeError, "out must be (packed, sf, sf_permuted)");
+                if (t->device() != o.t[0]->device()) raise(PyExc_ValueError, "out must be on the device of a");
+                if (t->element_size() != 1 || t->numel() < needed[i] || !t->is_non_overlapping_and_dense())
+                    raise(PyExc_ValueError, "out must be dense 1-byte tensors that hold the packed result, its scales and their permuted form");
                 ptr[i] = t->data_ptr();
             }
-            const int64_t m = p.m, n = p.n;
             e.output = NVFP4_OUT_NVFP4;
             e.out_packed = ptr[0];
             e.out_sf = ptr[1];

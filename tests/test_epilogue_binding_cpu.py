@@ -47,3 +47,16 @@ def test_a_bias_of_another_device_is_refused(lib, residual):
         assert _run(lib, f"call(bias={bias}, residual={residual})") == "ValueError bias must be on the device of a"
     # one of the same device goes on to the device, which is not there
     assert _run(lib, f"call(bias=tensor(256, dtype=torch.float16), residual={residual})").split()[0] in ("RuntimeError", "AcceleratorError")
+
+
+@pytest.mark.parametrize("place,bad,text", [
+    (0, "tensor(127, 128)", "hold"), (1, "tensor(128, 15)", "hold"), (2, "tensor(128, 15)", "hold"),
+    (0, "tensor(128, 128, dtype=torch.float16)", "hold"), (1, "tensor(128, 16, strides=[32, 1])", "hold"),
+    (0, "tensor(128, 128, device='cuda:62')", "device of a"), (1, "torch.zeros((128, 16), dtype=torch.uint8)", "device of a"),
+])
+def test_memory_that_does_not_hold_the_result_is_refused(lib, place, bad, text):
+    """The kernel would write past it, or to another device's address."""
+    out = ["tensor(128, 128)", "tensor(128, 16)", "tensor(128, 16)"]
+    out[place] = bad
+    answer = _run(lib, f"call(nvfp4_out=True, out=({', '.join(out)}))")
+    assert answer.startswith("ValueError") and text in answer
