@@ -54,8 +54,8 @@ struct DeviceCtx {
     int* status_dev = nullptr;
     size_t scratch_bytes = 0;
     std::atomic<bool> scratch_ready{false};   // scratch and counters are allocated and cleared
-    int max_pairs = -1;  // CTA pairs that can be co-resident (cluster occupancy), queried once
-    int expert_pairs = -1;   // the same for the experts' kernel
+    std::atomic<int> max_pairs{-1};      // CTA pairs that can be co-resident (cluster occupancy), queried by the first thread that needs it
+    std::atomic<int> expert_pairs{-1};   // the same for the experts' kernel
     std::atomic<bool> smem_attr_set[96] = {};   // by kernel variant: 0..26 the tiled kernels, 32.. the decode kernels, 72.. the experts' kernels
 };
 
