@@ -62,8 +62,15 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: O
     ties to the lowest index.  With ``groups`` > 1 only experts of the ``top_groups`` best of that many equal ranges can be
     chosen; a range is judged by its largest choice (``group_score="max"``) or the sum of its two largest (``"top2"``).  Weights are the
     scores without bias, divided by their sum if ``renormalize`` (0 where that is 0), times ``scale``.
-    An expert whose logit or bias is -inf or NaN cannot be chosen; a token with fewer than ``top_k`` others gets expert -1,
-    row -1 and weight 0 for the rest, so a padded token is one whose logits are all -inf.  Choices are made in 64 bits."""
+    An expert whose logit or bias is -inf or NaN cannot be chosen (+inf counts as the largest number); a token with fewer than
+    ``top_k`` others gets expert -1, row -1 and weight 0 for the rest, so a padded token is one whose logits are all -inf.
+
+    Choices are made in 64 bits.  Without ``bias``, and with groups judged by their largest choice if there are any, the logits
+    themselves are compared, whose order both scores keep; so experts are told apart there whose scores 64 bits hold as one
+    number (sigmoids from about 37 on, all 1; softmax scores more than 745 below the largest, all 0).  In every other case these
+    are a tie, which the lowest index takes: a ``bias`` of zeros takes the lowest of them, no ``bias`` the one of the largest logit.
+    Weights are made in 32 bits: that of a logit x is within ``(60 + 2 * abs(x - largest logit)) * 2**-24`` of its value by softmax,
+    within ``20 * 2**-24`` by sigmoid, as long as it is a normal number of 32 bits."""
     result = _lib.native().route(logits, top_k, _SCORING.get(scoring) or _choice(_SCORING, scoring, "scoring"), bias, groups, top_groups,
                                  _GROUP_SCORE.get(group_score) or _choice(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), scale)
     if type(result) is int:
