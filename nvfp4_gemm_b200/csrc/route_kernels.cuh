@@ -342,9 +342,15 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
 #pragma unroll
         for (int i = 0; i < VPL; ++i) key[i] = key_of(x[i]);
     } else {
-        // Errors of a score s, in units of 2^-24 of the largest: four for the exponential, one for its argument (times s, at most
-        // 0.37), five for the quotient, VPL + 5 for the softmax's total; then one of the choice.  Two compared choices: twice that;
-        // groups' sums of two: four times, and the roundings of the sums.
+        // Errors in units of u = 2^-24.
+        // Softmax.  exp(-d) by __expf is off by (4 + 3.35 d) u of itself (2 + 1.173 d ulp of two u, and d's own rounding): 4 u of the
+        // largest at most.  Its product with 1 / total adds one: 5 / total is what a choice has of its own.  All scores share the error of
+        // 1 / total: VPL + 5 for the additions, 4 for the quotient, and G for the exponentials that were summed, the mean of 4 + 3.35 d over the
+        // total.  G is largest where most of the total lies a few units below the largest logit: 10.1, 11.7, 13.4, 15.2, 17.0,
+        // 18.9 for 32, 64, ... 1024 experts.  What is shared counts by how far two scores differ, 1 / total at most.  With a rounding of
+        // `most` for either choice, two choices are off by (VPL + 19 + G) / total + 2 most; 2 (VPL + 16) / total + 2 most is taken,
+        // which is more as long as G < VPL + 13.  Sums of two choices each: twice that, and 4 most for the sums' own roundings.
+        // Sigmoid: 5.4 of a score of at most 1 (exponential, sum, quotient); 10 are taken.
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             // (an expert whose logit or bias is -inf or NaN: -inf)
@@ -501,7 +507,9 @@ __device__ __forceinline__ int choose(const RouteParams& p, const PlanParams& q,
         if (n > 32 && least <= 32 && !unsure_group) {
             // More than lanes: fewer lanes have anything than are to be chosen (few groups or experts are left, a lane's experts are neighbours), or
             // nearly as many are to be chosen as there are lanes.  A threshold that `least` to 32 keys are not below, by halves.
-            // (8192 tokens of 256 experts: 2 of 8 groups by logits 17.4 us, chosen in 64 bits 56; 24 and 32 of all 21.5 and 24.6, in 64 bits 53 and 64)
+            // (8192 tokens of 256 experts, by logits: 2 of 8 groups 17.4 us, chosen in 64 bits 56; 24 and 32 of all 21.4 and 24.5, in 64 bits 53 and 64.
+            // By scores 24 and 31 of all take 26.8 and 33.6; for 32 the 33rd would be needed too, one more than lanes, so where more than 32 can
+            // be chosen these are chosen in 64 bits: 72.5.)
             uint32_t low = floor_key, high = warp_max(best);      // more than 32 are not below low; fewer than least above high
 #pragma unroll 1
             while (low < high) {
