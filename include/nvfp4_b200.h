@@ -354,7 +354,8 @@ int nvfp4_plan_experts(const nvfp4_routing* routing, void* stream);
 /*
  * Token rows x (fp16, or bf16 if x_is_bf16; [tokens][k], 16-byte aligned, stride in elements a multiple of 8, 0 for one row for all) -> NVFP4 rows in
  * expert order: packed [tokens * top_k][k / 2] and sf.  A token is quantised once, by the rule of nvfp4_quantize(), and
- * written to each of its rows.  k a multiple of 64.
+ * written to each of its rows.  k a multiple of 64.  x has no scale of its own: beyond 6 * 448 it saturates, and where a block's maximum is
+ * below 6 * 2^-6 the block's scale is subnormal.
  */
 int nvfp4_quantize_routed(const void* x, int32_t x_is_bf16, int64_t x_row_stride, int32_t k, const nvfp4_routing* routing, void* packed,
                           int64_t packed_row_stride, void* sf, void* stream);
@@ -392,7 +393,7 @@ int nvfp4_expert_gemm(const nvfp4_expert_problem* problem, const nvfp4_routing* 
 
 /*
  * out[t] = residual[t] + sum_j weights[t][j] * y[row[t][j]], summed in fp32 in the order of j and rounded once.  y fp16 [y_rows][n]; out
- * and residual (or NULL) fp16, or bf16 if out_is_bf16, and may be the same memory.  A row outside [0, y_rows) adds
+ * and residual (or NULL) fp16, or bf16 if out_is_bf16, and may be the same memory; out is otherwise apart from what is read.  A row outside [0, y_rows) adds
  * nothing.  n a multiple of 8, 16-byte aligned rows; strides in elements.
  */
 int nvfp4_combine_experts(const void* y, int64_t y_row_stride, int32_t y_rows, const int32_t* row, const float* weights, int32_t tokens,

@@ -21,8 +21,9 @@
 // Bounds and figures (us; weights E x n x k, rows in all).  Few rows: HBM, each touched expert's weights once: 8 x 4096 x 7168 for one token
 // 20.7 (6.4 TB/s), 32 x 4096 x 4096 for 64 tokens x 4 45.4, 32 x 7168 x 2048 for 64 x 8 39.8 (6.6 TB/s).  Many rows: what the dense pair kernel
 // is bound by, and its rates: 65536 rows evenly over 32 experts, 4096 x 7168 693-703 (5.5 PFLOP/s; dense, 8 batches 677), 7168 x 2048 426-437 (dense 434); in
-// a loop the 1000 W limit holds the SM clock at 1.15 to 1.25 GHz.  The epilogue of a 256 x 256 tile takes 2.8 of its own, 3.3 with its stores, beside
-// 3.0 of MMAs at k = 2048.
+// a loop the 1000 W limit holds the SM clock at 1.15 to 1.25 GHz.  Short K: the epilogue of a 256 x 256 tile takes 2.8 of its own, 3.3 with its
+// stores, beside 3.0 of MMAs at k = 2048, and the next tile's MMAs wait for the half of it that reads what the accumulators share: 32768 rows,
+// 7168 x 2048, 229-232 at full clock, the tensor pipe 59 % busy.
 //
 // Every wait is bounded.  No load uses cluster multicast.
 #pragma once
@@ -196,6 +197,9 @@ __global__ void __launch_bounds__(ExpertSmem<CG, BT, STAGES, EPI_WARPS>::kThread
     if (warp == 0) {
         // ------------------------------------------------------------ producer
         if (ptx::elect_one()) {
+            // (also where an expert has several tiles of 32 rows: their blocks of the weights run side by side and meet in L2.  Weights that are
+            // kept gain nothing there, 512 x 8 of 256 experts of up to 292 rows, 2048 x 2048: 103.7 us, 103.8 so, and cost
+            // where there is one tile: 64 x 8 of 32, 4096 x 4096: 51.2, 44.8 so)
             const uint64_t pol_w = ptx::policy_evict_first();
             const uint64_t pol_x = ptx::policy_evict_last();
             uint32_t stage = 0, phase = 0;

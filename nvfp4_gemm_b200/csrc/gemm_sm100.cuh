@@ -86,7 +86,7 @@ struct GemmParams {
     // as fp16 to c, or re-quantised to NVFP4 (packed e2m1 + one e4m3 scale per 16 columns of a row,
     // the operand format of a following GEMM whose K is this GEMM's N).
     const __half* bias;          // [N] or null
-    const __half* residual;      // (EPI_EX == kEpiResidual) [L][M][N], added behind the activation
+    const __half* residual;      // (kHasResidual) [L][M][N], added behind the activation; kEpiResidualFp16 reads it through tma_res
     long long residual_row_stride, residual_batch_stride;       // elements
     int activation;              // kActNone / kActRelu / kActSilu
     int out_nvfp4;               // 0: fp16 to c; 1: packed + scales

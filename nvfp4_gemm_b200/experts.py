@@ -86,7 +86,11 @@ def plan(experts: torch.Tensor, num_experts: int) -> Routing:
 
 
 def quantize_routed(x: torch.Tensor, routing: Routing) -> RoutedRows:
-    """Token rows [T, K] (fp16 or bf16) -> NVFP4 rows in expert order, by the rule of ``nvfp4_quantize``."""
+    """Token rows [T, K] (fp16 or bf16) -> NVFP4 rows in expert order, by the rule of ``nvfp4_quantize``.
+
+    Rows are quantised as they are: beyond 6 * 448 = 2688 values saturate without notice, and where a block of 16 has its maximum below
+    6 * 2**-6 (0.094) its e4m3 scale is subnormal and loses bits.  Rows outside that range are the caller's to scale ahead of the call, and
+    to undo in the product's ``alpha``."""
     return RoutedRows(*_checked(_lib.native().quantize_routed(x, routing.rows, routing.plan, routing.num_experts)))
 
 
@@ -98,7 +102,8 @@ def expert_gemm(rows: RoutedRows, routing: Routing, w: torch.Tensor, w_sf: torch
     ``activation``: "none", "relu", "silu", or "swiglu" for silu(gate) * up with N/2 columns, gate and up rows of ``w`` alternating in
     groups of eight (:func:`interleave_gate_up`).  Returns fp16 [T * k, columns] in expert order (``out``, if given), or with
     ``nvfp4_out`` the :class:`RoutedRows` of the following product, quantised from the fp16-rounded values (``out_scale`` brings
-    small values into the scales' range; undo it in the following ``alpha``).  Rows of pairs that are none are left as they were."""
+    small values into the scales' range; undo it in the following ``alpha``).  Rows of pairs that are none are left as they were.
+    Results are fp16 whatever the type of the tokens, infinite beyond 65504; the NVFP4 form saturates at 2688.  "relu" keeps a NaN."""
     result = _checked(_lib.native().expert_gemm(rows[0], rows[1], routing.rows, routing.plan, routing.num_experts, w, w_sf, alpha, bias,
                                                 _choice(_ACTIVATIONS, activation, "activation"), out_scale, bool(nvfp4_out), out))
     return RoutedRows(*result) if nvfp4_out else result[0]
@@ -107,7 +112,8 @@ def expert_gemm(rows: RoutedRows, routing: Routing, w: torch.Tensor, w_sf: torch
 def combine(y: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, *, residual: Optional[torch.Tensor] = None,
             out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``residual[t] + sum_j weights[t, j] * y[rows[t, j]]``, summed in fp32 in the order of j and rounded once to ``dtype`` (fp16 or bf16;
-    default: the type of ``out``, else of ``residual``, else fp16).  A row outside ``y`` adds nothing; ``out`` may be ``residual``."""
+    default: the type of ``out``, else of ``residual``, else fp16).  A row outside ``y`` adds nothing; ``out`` may be ``residual``, and is
+    otherwise apart from what is read."""
     if dtype is None:
         dtype = out.dtype if out is not None else residual.dtype if residual is not None else torch.float16
     if dtype not in (torch.float16, torch.bfloat16):
@@ -120,7 +126,11 @@ def expert_layer(x: torch.Tensor, logits: torch.Tensor, up, down, top_k: int, *,
     """The feed-forward of a layer: route, quantise, up product (re-quantised), down product, combine, in x's type.
 
     ``up`` and ``down`` are (w, w_sf); ``router`` are the keywords of :func:`route`.  ``hidden_scale`` multiplies the hidden values
-    before they are quantised; it is the caller's to undo in ``down_alpha``.  ``residual`` (usually the layer's input) is added."""
+    before they are quantised; it is the caller's to undo in ``down_alpha``.  ``residual`` (usually the layer's input) is added.
+
+    Ranges are those of the steps, also where x is bf16: x is quantised as it is (:func:`quantize_routed`), and the experts' rows between
+    the down product and the combination are fp16, so what is beyond 65504 there is infinite in the result.  A smaller ``down_alpha``
+    and a larger ``scale`` of the router bring such rows into range."""
     r = route(logits, top_k, **router)
     hidden = expert_gemm(quantize_routed(x, r), r, up[0], up[1], alpha=up_alpha, bias=up_bias, activation=activation, out_scale=hidden_scale,
                          nvfp4_out=True)
