@@ -326,7 +326,8 @@ int nvfp4_routing_plan(int32_t tokens, int32_t top_k, int32_t experts, int32_t* 
  * top_k can, the rest are expert -1, row -1, weight 0.  Choices are made in 64 bits: they do not depend on how a
  * 32-bit sigmoid rounds.  Where logits are compared, those are told apart whose scores are one number in 64 bits (sigmoids from about
  * 37 on); with a bias, of zeros too, such experts are a tie for the lowest index.  Weights are made in 32 bits: that of a logit x is within
- * (60 + 2 |x - largest logit|) * 2^-24 of its value by softmax, within 20 * 2^-24 by sigmoid, as long as it is a normal number.
+ * (60 + 2 |x - largest logit|) * 2^-24 of its value by softmax, within 20 * 2^-24 by sigmoid, as long as it and the score that
+ * it is made of are normal numbers.
  */
 #define NVFP4_SCORE_SOFTMAX 0
 #define NVFP4_SCORE_SIGMOID 1

@@ -70,7 +70,7 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: O
     number (sigmoids from about 37 on, all 1; softmax scores more than 745 below the largest, all 0).  In every other case these
     are a tie, which the lowest index takes: a ``bias`` of zeros takes the lowest of them, no ``bias`` the one of the largest logit.
     Weights are made in 32 bits: that of a logit x is within ``(60 + 2 * abs(x - largest logit)) * 2**-24`` of its value by softmax,
-    within ``20 * 2**-24`` by sigmoid, as long as it is a normal number of 32 bits."""
+    within ``20 * 2**-24`` by sigmoid, as long as it and the score that it is made of are normal numbers of 32 bits."""
     result = _lib.native().route(logits, top_k, _SCORING.get(scoring) or _choice(_SCORING, scoring, "scoring"), bias, groups, top_groups,
                                  _GROUP_SCORE.get(group_score) or _choice(_GROUP_SCORE, group_score, "group_score"), bool(renormalize), scale)
     if type(result) is int:
