@@ -75,3 +75,26 @@ def test_nan_and_infinities_of_alpha_and_bias(ex, lib, oracle, tokens, activatio
     assert np.array_equal(q.packed.view(torch.uint8)[:used].cpu().numpy(), exp_packed)
     where = ref.sf_rows(r.offsets.cpu(), _tile_tokens(lib, tokens, top_k, experts))
     assert np.array_equal(ref.scales_of(q.sf, where, y.shape[1]).cpu().numpy(), exp_sf)
+
+
+@pytest.mark.parametrize("tokens", [20, 300])
+@pytest.mark.parametrize("activation", ["none", "relu", "silu"])
+def test_nan_among_the_block_scales(ex, lib, tokens, activation):
+    """A NaN scale of a block of weights makes its column NaN, one of a row's block the row."""
+    top_k, experts, n, k = 2, 4, 256, 512
+    r, rows, _ = _rows(ex, lib, tokens, top_k, experts, k, tokens + 1)
+    w, w_sf, _ = _weights(experts, n, k, 2)
+    offsets = r.offsets.tolist()
+    exp = ex.expert_gemm(rows, r, w, w_sf, activation=activation).clone()
+    row, col, block = 133, 9, 7                     # of expert 1, and the scale of k-block 7: atom 1, entry 3
+    w_sf.view(torch.uint8)[row % 32, (row % 128) // 32, row // 128, block % 4, block // 4, 1] = 0x7F
+    where = ref.sf_rows(r.offsets.cpu(), _tile_tokens(lib, tokens, top_k, experts))
+    at = int(where[col])                            # row 9 in expert order
+    atoms = rows.sf.view(torch.uint8).view(-1, k // 64, 32, 4, 4)
+    atoms[at // 128, block // 4, at % 32, (at % 128) // 32, block % 4] = 0x7F
+    y = ex.expert_gemm(rows, r, w, w_sf, activation=activation)
+    exp[offsets[1]:offsets[2], row] = NAN
+    exp[col] = NAN
+    used = offsets[-1]
+    assert torch.equal(torch.isnan(y[:used]), torch.isnan(exp[:used]))
+    assert torch.equal(torch.nan_to_num(y[:used], nan=0.0), torch.nan_to_num(exp[:used], nan=0.0))
